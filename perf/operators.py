@@ -5,10 +5,12 @@ clipping of gradients by their global norm.
 Parameters, gradients and moments of a case lie in flat buffers, each tensor at a multiple of 256 elements (a tensor of an
 allocator of its own starts at a multiple of 512 bytes as well); what lies between two tensors is zero and stays zero.
 
-8-bit moments: blocks of 256 elements of a tensor share an exponent E (int8); an element is a small float under it.
+8-bit moments: blocks of 256 elements of a tensor share an exponent E (an int8: E of exp_avg, E / 2 of exp_avg_sq, whose range is
+twice as wide); an element is a small float under it.
   exp_avg    sign, 4 bits f, 3 bits n     value  n 2^(E-17) (f = 0)   (8 + n) 2^(E-18+f)
   exp_avg_sq       5 bits f, 3 bits n     value  n 2^(E-33) (f = 0)   (8 + n) 2^(E-34+f)
-E is the exponent of the block's largest magnitude, one more where its significand is 1.875 or above.  The moment is rounded to 20
+E is the exponent of the block's largest magnitude, one more where its significand is 1.875 or above, and for exp_avg_sq one more
+where that is odd.  The moment is rounded to 20
 bits below the format's last place, then up with the probability of the rest, by 16 bits of a hash of (seed, step, tensor, block,
 element); a second moment that is not zero stays at least one unit of the last place."""
 import math
@@ -103,17 +105,19 @@ def _views(flat, s):
     return [flat[o:o + n].view(shape) for o, n, shape in s["places"]]
 
 
-def _exponents(largest, low):
-    """E of blocks whose largest magnitude is given (fp64)."""
+def _exponents(largest, unit):
+    """the int8 of blocks whose largest magnitude is given (fp64): E in units of 1 or 2"""
     f, k = torch.frexp(largest)
-    return torch.where(largest > 0, k - 1 + (f >= 0.9375).to(k.dtype), torch.full_like(k, low)).clamp(low, 127)
+    e = k - 1 + (f >= 0.9375).to(k.dtype)
+    return torch.where(largest > 0, (e + unit - 1) // unit, torch.full_like(k, -127)).clamp(-127, 127)
 
 
 def _encode_nearest(x, floor, top):
     """codes (no sign) and exponents of |x| [blocks, 256], to nearest: how the inputs of a case are made"""
     y = x.abs().double()
-    E = _exponents(y.amax(1), -127)
-    y = y * torch.exp2(-E.double())[:, None]
+    unit = 1 if floor == -14 else 2
+    E = _exponents(y.amax(1), unit)
+    y = y * torch.exp2(-unit * E.double())[:, None]
     _, k = torch.frexp(y)
     e = torch.where(y > 0, k - 1, torch.full_like(k, floor)).clamp(min=floor)
     n = torch.round(y * torch.exp2(3.0 - e.double()))
@@ -249,7 +253,7 @@ def _plain_step(s):
         g = s["G"].double()
         if case["clip"]:
             g = g * _factor(s, norm)
-        e1, e2 = s["E"][0].double(), s["E"][1].double()
+        e1, e2 = s["E"][0].double(), 2 * s["E"][1].double()
         m = _decode((s["M"] & 127), e1 - 17) * (1.0 - 2.0 * (s["M"] >> 7).double()) * b1 + g * (1 - b1)
         v = _decode(s["V"], e2 - 33) * b2 + g * g * (1 - b2)
         bits = _bits(s, k)
@@ -299,8 +303,9 @@ def _bits(s, step):
 def _round(y, floor, top, bits, keep=False):
     """codes, exponents and values of y >= 0 [blocks, 256]; the smallest normal's exponent under E is `floor`"""
     largest = y.amax(1)
-    E = _exponents(largest, -127)
-    scale = torch.exp2(E.double())[:, None]
+    unit = 1 if floor == -14 else 2
+    E = _exponents(largest, unit)
+    scale = torch.exp2(unit * E.double())[:, None]
     y = y / scale
     _, k = torch.frexp(y)
     e = torch.where(y > 0, k - 1, torch.full_like(k, floor)).clamp(min=floor)
@@ -340,7 +345,7 @@ def exact(case, seed):
             small = torch.arange(256, device=m.device)
             table = torch.where(small < 8, small.double(), (small % 8 + 8).double() * 2.0 ** (small // 8 - 1).double())
             sign = torch.where(m >= 128, -1.0, 1.0).double()
-            m, v = table[(m % 128).long()] * sign * 2.0 ** (E[0] - 17), table[v.long()] * 2.0 ** (E[1] - 33)
+            m, v = table[(m % 128).long()] * sign * 2.0 ** (E[0] - 17), table[v.long()] * 2.0 ** (2 * E[1] - 33)
         m = b1 * m.double() + (1 - b1) * g
         v = b2 * v.double() + (1 - b2) * g ** 2
         p = (1 - case["lr"] * case["weight_decay"]) * p - case["lr"] / (1 - b1 ** k) * m / ((v / (1 - b2 ** k)).sqrt() + case["eps"])
@@ -385,7 +390,8 @@ def _exact_round(y, r, octaves):
     E = torch.floor(torch.log2(torch.where(top > 0, top, torch.ones_like(top))))
     E = torch.where(2.0 ** E > top, E - 1, torch.where(2.0 ** (E + 1) <= top, E + 1, E))
     E = torch.where(top >= 1.875 * 2.0 ** E, E + 1, E)
-    E = torch.where(top > 0, E.clamp(-127, 127), torch.zeros_like(E))
+    E = torch.where(E % 2 == 1, E + 1, E) if octaves == 31 else E
+    E = torch.where(top > 0, E.clamp(-127, 127) if octaves == 15 else E.clamp(-254, 254), torch.zeros_like(E))
     k = torch.frexp(y).exponent.double() - 1                                # unit of the last place of each element's octave
     unit = 2.0 ** (torch.maximum(k, E - octaves + 1) - 3)
     t = torch.round(y / unit * 2.0 ** 20)
