@@ -722,6 +722,82 @@ size_t rfx_adam_tensor_bytes(void);      /* sizeof(rfx_adam_tensor), for foreign
 /* tensors: host array of `count` <= RFX_ADAM_MAX_TENSORS descriptors (read before the call returns). */
 int rfx_adam_step(const rfx_adam_tensor* tensors, int count, rfx_stream stream);
 
+/* ---- AdamW over many tensors, gradient norm and clipping -------------------------------------------------------
+ * The reference steps its optimizers with torch.optim.Adam only (mp_slam/slam.py:271-286); these are the entry points of a
+ * run that wants decoupled weight decay, moments in a quarter of the memory, or its gradients clipped:
+ *   m <- b1 m + (1-b1) g ; v <- b2 v + (1-b2) g^2 ; p <- p - lr wd p - lr/(1-b1^k) m / (sqrt(v)/sqrt(1-b2^k) + eps)
+ * with g the gradient times the clipping factor (if one is given).  Additive: the ABI number stays what it was.
+ *
+ * 8-bit moments (group.state_bits = 8): each run of RFX_ADAMW_BLOCK elements of a tensor shares one exponent E (an int8) per
+ * moment; an element is one byte under it,
+ *   exp_avg     sign, 4 bits f, 3 bits n:   n 2^(E-17) if f = 0, else (8+n) 2^(E-18+f)
+ *   exp_avg_sq        5 bits f, 3 bits n:   n 2^(E-33) if f = 0, else (8+n) 2^(E-34+f)
+ * E = floor(log2(largest magnitude of the run)), one more where the significand is >= 1.875; the byte holds E of exp_avg, and of
+ * exp_avg_sq -- whose range is twice as wide -- E / 2, rounded up; clamped to [-127, 127].  The byte -128: the run held a value
+ * that is not finite, and all of it reads as NaN.  A moment is rounded to 20 bits below the last place
+ * and then up with the probability of the rest, from 16 bits of a hash of (seed, step, index, run, element); a second moment
+ * > 0 never becomes 0.  The step itself uses the moments before they are rounded.                                          */
+#define RFX_F32  0
+#define RFX_BF16 1
+#define RFX_F16  2
+#define RFX_ADAMW_BLOCK 256
+typedef struct rfx_adamw_tensor {
+    void*        param;                 /* dev [n] of `dtype`, updated in place                                     */
+    const void*  grad;                  /* dev [n] of `dtype`                                                       */
+    void*        exp_avg;               /* dev [n]: float (state_bits 32) or bytes (8; 4-byte aligned)              */
+    void*        exp_avg_sq;            /* dev [n]: likewise                                                        */
+    int8_t*      exponents;             /* dev [2][ceil(n / RFX_ADAMW_BLOCK)]: of exp_avg, then of exp_avg_sq (8 only) */
+    float*       master;                /* dev [n] or NULL: the parameter in fp32, which is stepped in place of it    */
+    float*       step_dev;              /* dev [1] or NULL: the step count on the device (read, raised by one: for a   */
+                                        /* captured call); NULL: group.step                                         */
+    int64_t      n;
+    int32_t      group;                 /* which of `groups`                                                        */
+    uint32_t     index;                 /* of the parameter in its optimizer: keeps the tensors' roundings apart      */
+    int32_t      dtype;                 /* RFX_F32 / RFX_BF16 / RFX_F16 (master: the two 16-bit types only)          */
+    int32_t      reserved;
+} rfx_adamw_tensor;
+typedef struct rfx_adamw_group {
+    double       lr, beta1, beta2, eps, weight_decay;
+    const float* lr_dev;                /* dev [1] or NULL: the learning rate on the device (needs step_dev)          */
+    int64_t      step;                  /* k >= 1 of this step (tensors without step_dev)                           */
+    uint32_t     seed;                  /* of the 8-bit roundings                                                   */
+    int32_t      state_bits;            /* 32 or 8                                                                  */
+    int32_t      maximize;              /* step along the gradient instead of against it                            */
+    int32_t      reserved;
+} rfx_adamw_group;
+size_t rfx_adamw_tensor_bytes(void);
+size_t rfx_adamw_group_bytes(void);
+/* tensors / groups: host arrays of any length (read before the call returns); few launches for all of them.  Tensors of one
+ * call that share parameter memory are stepped one after the other.  clip: dev [2] as rfx_grad_norm writes it, or NULL.
+ * workspace: dev, 16-byte aligned, >= rfx_adamw_workspace_bytes(count) where a tensor has step_dev, else NULL.              */
+size_t rfx_adamw_workspace_bytes(int count);
+int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_group* groups, int n_groups, const double* clip,
+                   void* workspace, size_t workspace_bytes, rfx_stream stream);
+/* fp32 values of 8-bit moments (what a checkpoint in 32 bits or a look at the state needs), all tensors in few launches. */
+typedef struct rfx_moment_tensor {
+    const uint8_t* exp_avg;             /* dev [n], 4-byte aligned */
+    const uint8_t* exp_avg_sq;
+    const int8_t*  exponents;           /* dev [2][ceil(n / RFX_ADAMW_BLOCK)] */
+    float*         out_avg;             /* dev [n] */
+    float*         out_avg_sq;
+    int64_t        n;
+} rfx_moment_tensor;
+int rfx_adamw_moments(const rfx_moment_tensor* tensors, int count, rfx_stream stream);
+/* Norm of all gradients together and the factor that brings it under max_norm:
+ *   norm_type 2: N = sqrt(sum g^2), summed in fp64 in an order that depends on the sizes only; 0: N = max |g| (NaN if one is)
+ *   clip[0] = N, clip[1] = min(1, max_norm / (N + 1e-6)); norm32 (or NULL) gets N in fp32.
+ * rfx_grad_scale multiplies the gradients by clip[1], in place; with a factor of 1 nothing is written.                     */
+typedef struct rfx_grad_tensor {
+    void*   grad;                       /* dev [n] */
+    int64_t n;
+    int32_t dtype;
+    int32_t reserved;
+} rfx_grad_tensor;
+size_t rfx_grad_norm_workspace_bytes(const rfx_grad_tensor* tensors, int count);
+int rfx_grad_norm(const rfx_grad_tensor* tensors, int count, int norm_type, double max_norm, double* clip, float* norm32,
+                  void* workspace, size_t workspace_bytes, rfx_stream stream);
+int rfx_grad_scale(const rfx_grad_tensor* tensors, int count, const double* clip, rfx_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -43,6 +43,31 @@ class AdamTensor(C.Structure):
 
 
 ADAM_MAX_TENSORS = 16
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("exponents", C.c_void_p),
+                ("master", C.c_void_p), ("step_dev", C.c_void_p), ("n", C.c_int64), ("group", C.c_int32), ("index", C.c_uint32),
+                ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class AdamwGroup(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+                ("lr_dev", C.c_void_p), ("step", C.c_int64), ("seed", C.c_uint32), ("state_bits", C.c_int32), ("maximize", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
+class MomentTensor(C.Structure):
+    _fields_ = [("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("exponents", C.c_void_p), ("out_avg", C.c_void_p),
+                ("out_avg_sq", C.c_void_p), ("n", C.c_int64)]
+
+
+class GradTensor(C.Structure):
+    _fields_ = [("grad", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+ADAMW_BLOCK = 256           # RFX_ADAMW_BLOCK: elements that share an exponent in 8-bit moments
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # RFX_F32, RFX_BF16, RFX_F16
 LOSS_WS_DOUBLES = 2048      # RFX_LOSS_WS_DOUBLES
 # rfx_ba_desc.stage_events (RFX_BA_EV_*): entry i is recorded behind the last launch of stage i
 BA_STAGE_EVENTS = 10
@@ -184,6 +209,14 @@ PROTOTYPES = {
     "rfx_ba_desc_bytes": (C.c_size_t, []),
     "rfx_adam_tensor_bytes": (C.c_size_t, []),
     "rfx_adam_step": (_i, [C.POINTER(AdamTensor), C.c_int, _P]),
+    "rfx_adamw_tensor_bytes": (C.c_size_t, []),
+    "rfx_adamw_group_bytes": (C.c_size_t, []),
+    "rfx_adamw_workspace_bytes": (C.c_size_t, [_i]),
+    "rfx_adamw_step": (_i, [_P, _i, _P, _i, _P, _P, _sz, _P]),
+    "rfx_adamw_moments": (_i, [_P, _i, _P]),
+    "rfx_grad_norm_workspace_bytes": (C.c_size_t, [_P, _i]),
+    "rfx_grad_norm": (_i, [_P, _i, _i, C.c_double, _P, _P, _P, _sz, _P]),
+    "rfx_grad_scale": (_i, [_P, _i, _P, _P]),
     "rfx_ba_workspace_bytes": (C.c_size_t, [_l, _i, _i, _i, _i]),
     "rfx_ba_forward_backward": (_i, [C.POINTER(BaDesc), _P, C.c_size_t, _P]),
     "rfx_ba_workspace_layout": (_i, [_l, _i, _i, _i, _i, C.POINTER(C.c_size_t), _i]),
@@ -230,6 +263,8 @@ def load() -> C.CDLL:
         raise RfxError("librfx.so ABI version mismatch")
     if lib.rfx_adam_tensor_bytes() != C.sizeof(AdamTensor):
         raise RfxError("rfx_adam_tensor layout mismatch between librfx.so and _lib.AdamTensor")
+    if lib.rfx_adamw_tensor_bytes() != C.sizeof(AdamwTensor) or lib.rfx_adamw_group_bytes() != C.sizeof(AdamwGroup):
+        raise RfxError("rfx_adamw_tensor / rfx_adamw_group layout mismatch between include/rfx.h and remixfusion_amd/_lib.py")
     if lib.rfx_ba_desc_bytes() != C.sizeof(BaDesc):
         raise RfxError("rfx_ba_desc layout mismatch between include/rfx.h and remixfusion_amd/_lib.py")
     if lib.rfx_ba_shard_bytes() != C.sizeof(BaShard):

@@ -1,4 +1,5 @@
-"""Adam for the mapper's two optimizers, stepped by one librfx launch (rfx_adam_step).
+"""Adam for the mapper's two optimizers, stepped by one librfx launch (rfx_adam_step); AdamW over many tensors with its moments in
+32 or in 8 bits (rfx_adamw_step) and clipping by the gradients' global norm (rfx_grad_norm, rfx_grad_scale).
 
 Reference: ``optim.Adam(trainable_parameters, betas=(0.9, 0.99))`` / ``optim.Adam(rba_parameter, ...)`` in
 mp_slam/slam.py:271-286, stepped in mp_slam/mapper.py:416-418 and :497-499.  This is a ``torch.optim.Adam`` (same
@@ -8,7 +9,9 @@ maximize, closures that need grad mode) takes torch's own implementation.
 """
 import ctypes as C
 import math
+from operator import is_
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -132,3 +135,510 @@ class Adam(torch.optim.Adam):
                     with torch.cuda.device(dev):
                         _lib.check(lib.rfx_adam_step(arr, len(part), stream), "rfx_adam_step")
         return loss
+
+
+_GRAD_ROW = np.dtype(_lib.GradTensor)
+_TENSOR_ROW = np.dtype(_lib.AdamwTensor)
+_size, _stride, _ptr = torch.Tensor.size, torch.Tensor.stride, torch.Tensor.data_ptr
+
+
+def _address(rows):
+    return rows.__array_interface__["data"][0]
+
+
+def _same_memory_order(a, b):
+    """whether two tensors of one shape hold element i of memory for the same place (both dense, equal strides)"""
+    return a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous())
+
+
+def _dense(t):
+    """no element twice, no gap: any order of dimensions"""
+    if t.is_contiguous():
+        return True
+    n = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+def _overlaps_itself(t):
+    return any(st == 0 and sz > 1 for st, sz in zip(t.stride(), t.shape))
+
+
+class _on:
+    """the device that a call's launches go to, as the current one"""
+
+    def __init__(self, device):
+        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *a):
+        if self.guard is not None:
+            self.guard.__exit__(*a)
+
+
+def _check_grad(g):
+    if g.layout is not torch.strided:
+        raise _lib.RfxError("sparse gradients are not supported")
+    if g.dtype not in _lib.DTYPES:
+        raise _lib.RfxError(f"gradients of type {g.dtype} are not supported: float32, bfloat16 or float16")
+    if _overlaps_itself(g):
+        raise _lib.RfxError("a gradient whose elements share memory (an expanded tensor) is not supported")
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ as two passes of librfx kernels: the norm N of all gradients together (2-norm, summed in
+    fp64 in an order that depends on sizes only, or the largest magnitude with norm_type=inf), then every gradient times
+    min(1, max_norm / (N + 1e-6)) in place -- nothing is written where that is 1.  Returns N, an fp32 scalar on the gradients'
+    device; the host does not wait for it unless error_if_nonfinite asks (RuntimeError before anything is scaled).  A factor that is
+    not finite is applied as it is: an infinite norm makes zeros (and NaN of what was infinite), a NaN makes NaN.  One device;
+    float32 / bfloat16 / float16 gradients, mixed freely.  Gradients on the CPU take torch's own function."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    max_norm, norm_type = float(max_norm), float(norm_type)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm has to be a number >= 0: {max_norm}")
+    if not grads:
+        return torch.tensor(0.0)
+    if not any(g.is_cuda for g in grads):
+        return torch.nn.utils.clip_grad_norm_(parameters, max_norm, norm_type, error_if_nonfinite)
+    if norm_type not in (2.0, math.inf):
+        raise _lib.RfxError(f"norm_type {norm_type}: only 2 and inf are supported")
+    dev = grads[0].device
+    for g in grads:
+        _check_grad(g)
+        if g.device != dev:
+            raise _lib.RfxError("gradients on different devices: clip them device by device")
+    flat = [g if _dense(g) else g.contiguous() for g in grads]
+    rows = np.zeros(len(flat), _GRAD_ROW)
+    rows["grad"], rows["n"], rows["dtype"] = list(map(_ptr, flat)), [g.numel() for g in flat], [_lib.DTYPES[g.dtype] for g in flat]
+    lib, at = _lib.load(), _address(rows)
+    with _on(dev):
+        stream = _lib.stream_ptr(dev)
+        ws = torch.empty(2 + lib.rfx_grad_norm_workspace_bytes(at, len(rows)) // 8, dtype=torch.float64, device=dev)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        clip = ws.data_ptr()
+        _lib.check(lib.rfx_grad_norm(at, len(rows), 2 if norm_type == 2.0 else 0, max_norm, clip, norm.data_ptr(), clip + 16,
+                                     ws.numel() * 8 - 16, stream), "rfx_grad_norm")
+        if error_if_nonfinite and not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"the norm of the gradients is not finite ({float(norm)}), so they cannot be clipped")
+        _lib.check(lib.rfx_grad_scale(at, len(rows), clip, stream), "rfx_grad_scale")
+        for g, f in zip(grads, flat):
+            if f is not g:
+                g.copy_(f)
+    return norm
+
+
+class _Plan:
+    """what the descriptors of one step hold that stays the same from step to step: the parameters that have a gradient, on one
+    device, with their state.  Checked against the optimizer at every step and built again when anything of it changed."""
+    __slots__ = ("device", "params", "ptrs", "shapes", "strides", "dtypes", "states", "parts", "rows", "at", "grads", "grads_at",
+                 "ws_bytes", "index", "spans", "settings", "groups", "flat", "counted", "ordered")
+
+
+class AdamW(torch.optim.AdamW):
+    """torch.optim.AdamW (decoupled weight decay) whose step is one librfx call over all tensors.  Device parameters in float32,
+    bfloat16 or float16; on the CPU torch's own step runs (32-bit moments, no clipping).  Moments are fp32 whatever the parameter's
+    type: state[p] = {"step", "exp_avg", "exp_avg_sq"}.  Beyond torch's arguments, the first three also per parameter group:
+
+    state_bits      32, or 8: moments of one byte under an exponent per 256 elements (include/rfx.h has the format), a quarter of the
+                    memory and 16 instead of 28 bytes of traffic per fp32 parameter; state[p] holds uint8 "exp_avg", "exp_avg_sq" and
+                    int8 "exponents" [2, ceil(n / 256)].  Rounded stochastically from a hash of (seed, step, parameter, element): the same
+                    run gives the same bits.  A value that is not finite makes its 256 neighbours NaN at the next step.
+    master_weights  bfloat16 / float16 parameters are stepped in an fp32 copy, state[p]["master"], and rounded once.
+    seed            of the 8-bit roundings.
+    max_grad_norm   scale the gradients by min(1, max_grad_norm / (N + 1e-6)), N their global 2-norm, on the way into the moments: the
+                    gradients themselves stay as they are.  `grad_norm` is N of the last step (fp32 scalar on the device).
+    capturable      the step count lives on the device and lr may be a device scalar: step() can be captured into a graph (after one
+                    step or prepare(), which create the state).  Without it a capture is refused.
+
+    moments() gives the moments as fp32 tensors.  amsgrad and differentiable are refused."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=False, *, maximize=False,
+                 capturable=False, state_bits=32, master_weights=False, seed=0, max_grad_norm=None, differentiable=False,
+                 foreach=None, fused=None):
+        if amsgrad or differentiable:
+            raise ValueError("remixfusion_amd.optim.AdamW has no amsgrad and no differentiable step")
+        if isinstance(lr, torch.Tensor) and not capturable:
+            raise ValueError("a tensor lr needs capturable=True")
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
+            raise ValueError(f"max_grad_norm has to be None or a number >= 0: {max_grad_norm}")
+        self._own = {"state_bits": state_bits, "master_weights": master_weights, "seed": seed}
+        self._reset()
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize, capturable=capturable)
+        self.defaults.update(self._own, max_grad_norm=None if max_grad_norm is None else float(max_grad_norm))
+
+    def _reset(self):
+        self._plans, self._steps, self._dev_steps = {}, None, {}
+        self.grad_norm = None
+
+    _patch_step_function = Adam._patch_step_function
+    _hooked = Adam._hooked
+
+    @property
+    def max_grad_norm(self):
+        return self.defaults["max_grad_norm"]
+
+    @max_grad_norm.setter
+    def max_grad_norm(self, value):
+        if value is not None and not float(value) >= 0.0:
+            raise ValueError(f"max_grad_norm has to be None or a number >= 0: {value}")
+        self.defaults["max_grad_norm"] = None if value is None else float(value)
+
+    def add_param_group(self, group):
+        own = self._own
+        for key, value in own.items():
+            group.setdefault(key, value)
+        if group["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits is 32 or 8: {group['state_bits']}")
+        if not isinstance(group["seed"], int) or not 0 <= group["seed"] < 1 << 32:
+            raise ValueError(f"seed is a whole number of 32 bits: {group['seed']}")
+        super().add_param_group(group)
+        ids = [id(p) for p in self.param_groups[-1]["params"]]
+        if len(set(ids)) != len(ids):
+            self.param_groups.pop()
+            raise ValueError("a parameter stands twice in a group")
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "max_grad_norm" in self.defaults:                 # a copy or an unpickled optimizer: only the three dicts came along
+            self._own = {k: self.defaults[k] for k in ("state_bits", "master_weights", "seed")}
+        self._reset()
+        for g in self.param_groups:
+            for k, v in self._own.items():
+                g.setdefault(k, v)
+
+    # ---- state ------------------------------------------------------------------------------------------------------------
+    def load_state_dict(self, state_dict):
+        """as torch's, but moments and master weights keep their own types (torch casts them to the parameter's); a dict of
+        torch.optim.AdamW fits groups with 32-bit moments"""
+        seen, mine = [], [{k: g[k] for k in self._own} for g in self.param_groups]
+        hook = self.register_load_state_dict_pre_hook(lambda opt, d: seen.append(d))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
+        for g, saved, old in zip(self.param_groups, seen[0]["param_groups"], mine):
+            g.update({k: v for k, v in old.items() if k not in saved})
+            for i, p in zip(saved["params"], g["params"]):
+                st = seen[0]["state"].get(i)
+                if st:
+                    for key in ("exp_avg", "exp_avg_sq", "exponents", "master"):
+                        if key in st:
+                            self.state[p][key] = st[key].to(device=p.device)
+                    if p.is_cuda:
+                        self._check_state(p, g)
+
+    def _check_state(self, p, g):
+        """brings a state that came from outside to the types and the memory order a step needs, or refuses it"""
+        st, eight = self.state[p], g["state_bits"] == 8
+        missing = [k for k in ("step", "exp_avg", "exp_avg_sq") + (("exponents",) if eight else ()) if k not in st]
+        if missing:
+            raise _lib.RfxError(f"the state of a parameter lacks {', '.join(missing)}")
+        order = p if _dense(p) else None                     # whose memory order the state has
+        for key in ("exp_avg", "exp_avg_sq"):
+            t = st[key]
+            if tuple(t.shape) != tuple(p.shape) or not t.is_cuda or t.device != p.device:
+                raise _lib.RfxError(f"{key} of shape {tuple(t.shape)} on {t.device} for a parameter of shape {tuple(p.shape)} on {p.device}")
+            if (t.dtype == torch.uint8) != eight:
+                raise _lib.RfxError(f"{key} of type {t.dtype} for a group with state_bits={g['state_bits']}: moments are not converted on the way in")
+            if order is None and _dense(t) and not eight:
+                order = t
+            fits = _dense(t) and (_same_memory_order(t, order) if order is not None else t.is_contiguous())
+            if eight:
+                if not fits:
+                    raise _lib.RfxError(f"8-bit {key} with strides {tuple(t.stride())} for a parameter with {tuple(p.stride())}: its "
+                                        "exponents belong to runs of another memory order")
+                if t.data_ptr() & 3:
+                    st[key] = t.clone()
+            elif not fits or t.dtype != torch.float32:
+                st[key] = torch.empty_like(t.contiguous() if order is None else order, dtype=torch.float32).copy_(t)
+            order = st[key] if order is None else order
+        if eight:
+            e = st["exponents"]
+            if e.dtype != torch.int8 or tuple(e.shape) != (2, -(-p.numel() // _lib.ADAMW_BLOCK)) or e.device != p.device:
+                raise _lib.RfxError(f"exponents of type {e.dtype}, shape {tuple(e.shape)} on {e.device}: int8 [2, {-(-p.numel() // _lib.ADAMW_BLOCK)}] is needed")
+            st["exponents"] = e.contiguous()
+        if g["master_weights"] and p.dtype != torch.float32:
+            w = st.get("master")
+            if w is None or tuple(w.shape) != tuple(p.shape) or w.dtype != torch.float32 or w.device != p.device or not (
+                    _dense(w) and _same_memory_order(w, st["exp_avg"])):
+                if w is not None and tuple(w.shape) != tuple(p.shape):
+                    raise _lib.RfxError(f"master of shape {tuple(w.shape)} for a parameter of shape {tuple(p.shape)}")
+                st["master"] = torch.empty_like(st["exp_avg"], dtype=torch.float32).copy_(p if w is None else w)
+
+    def _new_state(self, p, g):
+        st = self.state[p]
+        st["step"] = torch.tensor(0.0, dtype=torch.float32)
+        kind = torch.uint8 if g["state_bits"] == 8 else torch.float32
+        st["exp_avg"] = torch.zeros_like(p, dtype=kind, memory_format=torch.preserve_format)
+        st["exp_avg_sq"] = torch.zeros_like(st["exp_avg"])
+        if g["state_bits"] == 8:                              # the exponent of a run of zeros is the least one
+            st["exponents"] = torch.full((2, -(-p.numel() // _lib.ADAMW_BLOCK)), -127, dtype=torch.int8, device=p.device)
+        if g["master_weights"] and p.dtype != torch.float32:
+            st["master"] = torch.empty_like(st["exp_avg"], dtype=torch.float32).copy_(p)
+
+    @torch.no_grad()
+    def prepare(self):
+        """create the state of every device parameter now (what the first step() would do on its way); needed before a step is
+        captured into a graph"""
+        every = [(p, i, gi) for i, (gi, p) in enumerate((gi, p) for gi, g in enumerate(self.param_groups) for p in g["params"])
+                 if p.is_cuda and p.requires_grad]
+        if every:
+            self._build(every)
+
+    @torch.no_grad()
+    def moments(self):
+        """(exp_avg, exp_avg_sq) of all parameters, in their order, as fp32 tensors: the state's own tensors where moments are held
+        in 32 bits, the values of the codes where in 8, zeros where there is no state yet"""
+        avg, avg_sq, decode = [], [], {}
+        for g in self.param_groups:
+            for p in g["params"]:
+                st = self.state.get(p)
+                if not st:
+                    avg.append(torch.zeros_like(p, dtype=torch.float32))
+                    avg_sq.append(torch.zeros_like(p, dtype=torch.float32))
+                elif st["exp_avg"].dtype != torch.uint8:
+                    avg.append(st["exp_avg"])
+                    avg_sq.append(st["exp_avg_sq"])
+                else:
+                    self._check_state(p, g)
+                    m, v = st["exp_avg"], st["exp_avg_sq"]
+                    avg.append(torch.empty_like(m, dtype=torch.float32))
+                    avg_sq.append(torch.empty_like(v, dtype=torch.float32))
+                    decode.setdefault(p.device, []).append(_lib.MomentTensor(m.data_ptr(), v.data_ptr(), st["exponents"].data_ptr(),
+                                                                             avg[-1].data_ptr(), avg_sq[-1].data_ptr(), m.numel()))
+        for dev, ts in decode.items():
+            with _on(dev):
+                _lib.check(_lib.load().rfx_adamw_moments((_lib.MomentTensor * len(ts))(*ts), len(ts), _lib.stream_ptr(dev)), "rfx_adamw_moments")
+        return avg, avg_sq
+
+    # ---- the step ---------------------------------------------------------------------------------------------------------
+    def _counters(self, n):
+        """the step counts of all parameters as one host array; state[p]["step"] is its element's view"""
+        if self._steps is None or len(self._steps[0]) != n:
+            t = torch.zeros(n, dtype=torch.float32)
+            self._steps = (t.numpy(), list(t))
+        return self._steps
+
+    def _build(self, every):
+        """plans for (parameter, its place in the optimizer, its group): states made or checked, one plan per device"""
+        capturing = torch.cuda.is_current_stream_capturing()
+        total = sum(len(g["params"]) for g in self.param_groups)
+        _, views = self._counters(total)
+        by_device = {}
+        for p, i, gi in every:
+            by_device.setdefault(p.device, []).append((p, i, gi))
+        for dev, part in by_device.items():
+            for p, i, gi in part:
+                g = self.param_groups[gi]
+                if p.dtype not in _lib.DTYPES:
+                    raise _lib.RfxError(f"parameters of type {p.dtype} are not supported: float32, bfloat16 or float16")
+                if _overlaps_itself(p):
+                    raise _lib.RfxError("a parameter whose elements share memory (an expanded tensor) is not supported")
+                st = self.state.get(p)
+                if not st:
+                    if capturing:
+                        raise _lib.RfxError("the state is created by the first step() or prepare(): call it before capturing")
+                    self._new_state(p, g)
+                else:
+                    self._check_state(p, g)
+                st = self.state[p]
+                if g["capturable"]:
+                    have = self._dev_steps.get(dev)
+                    if have is None or len(have) != total:
+                        if capturing:
+                            raise _lib.RfxError("the state is created by the first step() or prepare(): call it before capturing")
+                        have = self._dev_steps[dev] = list(torch.zeros(total, dtype=torch.float32, device=dev))
+                    view = have[i]
+                else:
+                    view = views[i]
+                if st["step"] is not view:
+                    if capturing:
+                        raise _lib.RfxError("the state is created by the first step() or prepare(): call it before capturing")
+                    view.copy_(st["step"].detach().reshape(()))
+                    st["step"] = view
+        self._plans = {dev: self._plan(dev, part) for dev, part in by_device.items()}
+        self._order, self._values = [p for p, _, _ in every], list(self.state.values())
+
+    def _plan(self, dev, part):
+        q = _Plan()
+        q.device = dev
+        q.params = [p for p, _, _ in part]
+        q.index = np.array([i for _, i, _ in part])
+        q.states = [self.state[p] for p in q.params]
+        q.parts = [x for st in q.states for x in st.values()]
+        q.ptrs, q.flat = list(map(_ptr, q.params)), list(map(_ptr, q.parts))
+        q.shapes, q.dtypes = list(map(_size, q.params)), [p.dtype for p in q.params]
+        q.strides = list(map(_stride, q.params))
+        q.ordered = all(p.stride() == st["exp_avg"].stride() for p, st in zip(q.params, q.states))
+        q.grads = np.zeros(len(part), _GRAD_ROW)
+        q.grads["n"] = [p.numel() for p in q.params]
+        q.grads["dtype"] = [_lib.DTYPES[t] for t in q.dtypes]
+        q.grads_at = _address(q.grads)
+        q.ws_bytes = None
+        q.rows = np.zeros(len(part), _TENSOR_ROW)
+        q.at = _address(q.rows)
+        q.spans, q.settings, q.counted = [], [], False
+        for k, (p, i, gi) in enumerate(part):
+            g, st, r = self.param_groups[gi], q.states[k], q.rows[k]
+            if not q.spans or q.spans[-1][0] != gi:
+                q.spans.append([gi, k, k])
+                q.settings.append((g["state_bits"], g["master_weights"], g["capturable"]))
+            q.spans[-1][2] = k + 1
+            r["param"], r["exp_avg"], r["exp_avg_sq"] = q.ptrs[k], st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()
+            if g["state_bits"] == 8:
+                r["exponents"] = st["exponents"].data_ptr()
+            if g["master_weights"] and p.dtype != torch.float32:
+                r["master"] = st["master"].data_ptr()
+            if g["capturable"]:
+                r["step_dev"], q.counted = st["step"].data_ptr(), True
+            r["n"], r["group"], r["index"], r["dtype"] = p.numel(), len(q.spans) - 1, i, _lib.DTYPES[p.dtype]
+        q.groups = (_lib.AdamwGroup * len(q.spans))()
+        return q
+
+    def _holds(self, q):
+        """whether a plan still says where everything is"""
+        parts = [x for st in q.states for x in st.values()]
+        return (len(parts) == len(q.parts) and all(map(is_, parts, q.parts)) and list(map(_ptr, parts)) == q.flat
+                and list(map(_ptr, q.params)) == q.ptrs and list(map(_stride, q.params)) == q.strides
+                and list(map(_size, q.params)) == q.shapes and [p.dtype for p in q.params] == q.dtypes
+                and [self._settings(gi) for gi, _, _ in q.spans] == q.settings)
+
+    def _settings(self, gi):
+        g = self.param_groups[gi]
+        return g["state_bits"], g["master_weights"], g["capturable"]
+
+    def step(self, closure=None):
+        if self._hooked():
+            return torch.optim.Optimizer.profile_hook_step(type(self)._step_impl)(self, closure)
+        out = self._step_impl(closure)
+        self._optimizer_step_code()
+        return out
+
+    @torch.no_grad()
+    def _step_impl(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        params = [p for g in self.param_groups for p in g["params"] if p.grad is not None]
+        if not params:
+            return loss
+        if not params[0].is_cuda:
+            self._cpu_step(params)
+            return loss
+        if not self._plans or len(params) != len(self._order) or not all(map(is_, params, self._order)) \
+                or len(self.state) != len(self._values) or not all(map(is_, self.state.values(), self._values)) \
+                or not all(map(self._holds, self._plans.values())):
+            if not all(p.is_cuda for p in params):
+                raise _lib.RfxError("parameters on the CPU and on a device in one optimizer are not supported")
+            self._build([(p, i, gi) for i, (gi, p) in enumerate((gi, p) for gi, g in enumerate(self.param_groups) for p in g["params"])
+                         if p.grad is not None])
+        if self.max_grad_norm is not None and len(self._plans) > 1:
+            raise _lib.RfxError("max_grad_norm needs all parameters on one device")
+        for q in self._plans.values():
+            self._launch(q)
+        return loss
+
+    def _cpu_step(self, params):
+        if any(p.is_cuda for p in params):
+            raise _lib.RfxError("parameters on the CPU and on a device in one optimizer are not supported")
+        if self.max_grad_norm is not None or any(g["state_bits"] != 32 or g["master_weights"] for g in self.param_groups):
+            raise _lib.RfxError("8-bit moments, master weights and max_grad_norm need device parameters: there is no CPU path")
+        torch_step = torch.optim.AdamW.step
+        getattr(torch_step, "__wrapped__", torch_step)(self, None)
+
+    def _launch(self, q):
+        lib, dev = _lib.load(), q.device
+        grads = [p.grad for p in q.params]
+        late = None
+        rows, at, grows, grads_at = q.rows, q.at, q.grads, q.grads_at
+        try:
+            direct = q.ordered and list(map(_stride, grads)) == q.strides and list(map(_size, grads)) == q.shapes and [g.dtype for g in grads] == q.dtypes
+        except RuntimeError:                                   # a layout without strides
+            direct = False
+        if not direct:
+            rows, grows = rows.copy(), grows.copy()
+            at, grads_at = _address(rows), _address(grows)
+            grads, late = self._in_order(q, grads, rows)
+        grows["grad"] = rows["grad"] = list(map(_ptr, grads))
+        with _on(dev):
+            if not q.counted or any(not s[2] for s in q.settings):
+                if torch.cuda.is_current_stream_capturing():
+                    raise _lib.RfxError("a step without capturable=True cannot be captured: its step count would stand still")
+            groups = self._fill(q, rows)
+            stream = _lib.stream_ptr(dev)
+            clip = ws = None
+            if self.max_grad_norm is not None:
+                if q.ws_bytes is None:
+                    q.ws_bytes = lib.rfx_grad_norm_workspace_bytes(grads_at, len(grads))
+                buf = torch.empty(2 + q.ws_bytes // 8, dtype=torch.float64, device=dev)
+                self.grad_norm = torch.empty((), dtype=torch.float32, device=dev)
+                clip = buf.data_ptr()
+                _lib.check(lib.rfx_grad_norm(grads_at, len(grads), 2, self.max_grad_norm, clip, self.grad_norm.data_ptr(), clip + 16,
+                                             q.ws_bytes, stream), "rfx_grad_norm")
+            n_ws = 0
+            if q.counted:
+                n_ws = lib.rfx_adamw_workspace_bytes(len(grads))
+                ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
+            _lib.check(lib.rfx_adamw_step(at, len(grads), groups, len(groups), clip, None if ws is None else ws.data_ptr(), n_ws, stream),
+                       "rfx_adamw_step")
+            if late:
+                for p, x in late:
+                    p.copy_(x)
+
+    def _in_order(self, q, grads, rows):
+        """gradients (and parameters with gaps) brought to the memory order of their moments; `late`: what goes back afterwards"""
+        out, late = [], []
+        for k, (p, g, st) in enumerate(zip(q.params, grads, q.states)):
+            _check_grad(g)
+            if g.dtype != p.dtype or g.shape != p.shape or g.device != p.device:
+                raise _lib.RfxError(f"a gradient of type {g.dtype}, shape {tuple(g.shape)} on {g.device} for a parameter of type {p.dtype}, "
+                                    f"shape {tuple(p.shape)} on {p.device}")
+            m = st["exp_avg"]
+            if not _same_memory_order(p, m):
+                x = torch.empty_like(m, dtype=p.dtype).copy_(p)
+                late.append((p, x))
+                rows[k]["param"] = x.data_ptr()
+            out.append(g if _same_memory_order(g, m) else torch.empty_like(m, dtype=g.dtype).copy_(g))
+        return out, late
+
+    def _fill(self, q, rows):
+        """raises the host's step counts and writes what belongs to a parameter group; more entries where its counts differ"""
+        groups, n = q.groups, len(q.spans)
+        for k, (gi, lo, hi) in enumerate(q.spans):
+            g, e = self.param_groups[gi], groups[k]
+            lr = g["lr"]
+            if isinstance(lr, torch.Tensor):
+                if not g["capturable"] or not lr.is_cuda or lr.device != q.device or lr.dtype != torch.float32 or lr.numel() != 1:
+                    raise _lib.RfxError("a tensor lr needs capturable=True and has to be one float32 on the parameters' device")
+                e.lr_dev = lr.data_ptr()
+            else:
+                e.lr, e.lr_dev = lr, None
+            e.beta1, e.beta2 = g["betas"]
+            e.eps, e.weight_decay, e.seed, e.state_bits, e.maximize = g["eps"], g["weight_decay"], g["seed"], g["state_bits"], g["maximize"]
+            if g["capturable"]:
+                continue
+            steps = self._steps[0]
+            at = q.index[lo:hi]
+            now = steps[at] + 1.0
+            steps[at] = now
+            e.step = int(now[0])
+            if not (now == now[0]).all():                      # parameters that joined at different steps
+                counts = sorted({int(x) for x in now})
+                more = (_lib.AdamwGroup * (len(groups) + len(counts)))(*groups)
+                for j, c in enumerate(counts):
+                    more[len(groups) + j] = e
+                    more[len(groups) + j].step = c
+                    rows["group"][lo:hi][now == c] = len(groups) + j
+                groups = more
+            else:
+                rows["group"][lo:hi] = k
+        return groups
