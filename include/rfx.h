@@ -786,7 +786,8 @@ int rfx_adamw_moments(const rfx_moment_tensor* tensors, int count, rfx_stream st
 /* Norm of all gradients together and the factor that brings it under max_norm:
  *   norm_type 2: N = sqrt(sum g^2), summed in fp64 in an order that depends on the sizes only; 0: N = max |g| (NaN if one is)
  *   clip[0] = N, clip[1] = min(1, max_norm / (N + 1e-6)); norm32 (or NULL) gets N in fp32.
- * rfx_grad_scale multiplies the gradients by clip[1], in place; with a factor of 1 nothing is written.                     */
+ * rfx_grad_scale multiplies the gradients by clip[1], in place; with a factor of 1 nothing is written.  rfx_grad_clip is one after
+ * the other (a small set in one launch).  Gradients of one call that share memory are scaled one after the other.          */
 typedef struct rfx_grad_tensor {
     void*   grad;                       /* dev [n] */
     int64_t n;
@@ -795,6 +796,8 @@ typedef struct rfx_grad_tensor {
 } rfx_grad_tensor;
 size_t rfx_grad_norm_workspace_bytes(const rfx_grad_tensor* tensors, int count);
 int rfx_grad_norm(const rfx_grad_tensor* tensors, int count, int norm_type, double max_norm, double* clip, float* norm32,
+                  void* workspace, size_t workspace_bytes, rfx_stream stream);
+int rfx_grad_clip(const rfx_grad_tensor* tensors, int count, int norm_type, double max_norm, double* clip, float* norm32,
                   void* workspace, size_t workspace_bytes, rfx_stream stream);
 int rfx_grad_scale(const rfx_grad_tensor* tensors, int count, const double* clip, rfx_stream stream);
 

@@ -216,6 +216,7 @@ PROTOTYPES = {
     "rfx_adamw_moments": (_i, [_P, _i, _P]),
     "rfx_grad_norm_workspace_bytes": (C.c_size_t, [_P, _i]),
     "rfx_grad_norm": (_i, [_P, _i, _i, C.c_double, _P, _P, _P, _sz, _P]),
+    "rfx_grad_clip": (_i, [_P, _i, _i, C.c_double, _P, _P, _P, _sz, _P]),
     "rfx_grad_scale": (_i, [_P, _i, _P, _P]),
     "rfx_ba_workspace_bytes": (C.c_size_t, [_l, _i, _i, _i, _i]),
     "rfx_ba_forward_backward": (_i, [C.POINTER(BaDesc), _P, C.c_size_t, _P]),

@@ -689,6 +689,12 @@ int rfx_grad_norm(const rfx_grad_tensor* tensors, int count, int norm_type, doub
     return RFX_OK;
 }
 
+int rfx_grad_clip(const rfx_grad_tensor* tensors, int count, int norm_type, double max_norm, double* clip, float* norm32,
+                  void* workspace, size_t workspace_bytes, rfx_stream stream) {
+    const int rc = rfx_grad_norm(tensors, count, norm_type, max_norm, clip, norm32, workspace, workspace_bytes, stream);
+    return rc == RFX_OK ? rfx_grad_scale(tensors, count, clip, stream) : rc;
+}
+
 int rfx_grad_scale(const rfx_grad_tensor* tensors, int count, const double* clip, rfx_stream stream) {
     if (!grads_ok(tensors, count) || !clip) return RFX_ERR_ARG;
     GnArgs k;

@@ -9,10 +9,11 @@ maximize, closures that need grad mode) takes torch's own implementation.
 """
 import ctypes as C
 import math
+import struct
 from operator import is_
 
-import numpy as np
 import torch
+from torch.optim import optimizer as _torch_optimizer
 
 from . import _lib
 
@@ -137,13 +138,10 @@ class Adam(torch.optim.Adam):
         return loss
 
 
-_GRAD_ROW = np.dtype(_lib.GradTensor)
-_TENSOR_ROW = np.dtype(_lib.AdamwTensor)
-_size, _stride, _ptr = torch.Tensor.size, torch.Tensor.stride, torch.Tensor.data_ptr
-
-
-def _address(rows):
-    return rows.__array_interface__["data"][0]
+_size, _stride, _ptr, _numel, _get_device = (getattr(torch.Tensor, k) for k in ("size", "stride", "data_ptr", "numel", "get_device"))
+_is_contiguous = torch.Tensor.is_contiguous
+_capturing = torch._C._cuda_isCurrentStreamCapturing if hasattr(torch._C, "_cuda_isCurrentStreamCapturing") else (lambda: False)
+_TYPE_OF = _lib.DTYPES.get
 
 
 def _same_memory_order(a, b):
@@ -169,9 +167,10 @@ def _overlaps_itself(t):
 
 class _on:
     """the device that a call's launches go to, as the current one"""
+    __slots__ = ("guard",)
 
-    def __init__(self, device):
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    def __init__(self, index):
+        self.guard = None if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
     def __enter__(self):
         if self.guard is not None:
@@ -191,7 +190,12 @@ def _check_grad(g):
         raise _lib.RfxError("a gradient whose elements share memory (an expanded tensor) is not supported")
 
 
-@torch.no_grad()
+def _grad_rows(grads):
+    """rfx_grad_tensor descriptors of gradients of the known types"""
+    rows = [x for row in zip(map(_ptr, grads), map(_numel, grads), [_TYPE_OF(g.dtype) for g in grads]) for x in row]
+    return struct.pack("Qqi4x" * len(grads), *rows)
+
+
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ as two passes of librfx kernels: the norm N of all gradients together (2-norm, summed in
     fp64 in an order that depends on sizes only, or the largest magnitude with norm_type=inf), then every gradient times
@@ -206,40 +210,48 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         raise ValueError(f"max_norm has to be a number >= 0: {max_norm}")
     if not grads:
         return torch.tensor(0.0)
-    if not any(g.is_cuda for g in grads):
+    index = max(map(_get_device, grads))
+    if index < 0:
         return torch.nn.utils.clip_grad_norm_(parameters, max_norm, norm_type, error_if_nonfinite)
     if norm_type not in (2.0, math.inf):
         raise _lib.RfxError(f"norm_type {norm_type}: only 2 and inf are supported")
+    if any(g.layout is not torch.strided or g.dtype not in _lib.DTYPES for g in grads):
+        for g in grads:
+            _check_grad(g)
+    if min(map(_get_device, grads)) != index:
+        raise _lib.RfxError("gradients on different devices: clip them device by device")
+    flat = grads
+    if not all(map(_is_contiguous, grads)):
+        for g in grads:
+            _check_grad(g)
+        flat = [g if _dense(g) else g.contiguous() for g in grads]
     dev = grads[0].device
-    for g in grads:
-        _check_grad(g)
-        if g.device != dev:
-            raise _lib.RfxError("gradients on different devices: clip them device by device")
-    flat = [g if _dense(g) else g.contiguous() for g in grads]
-    rows = np.zeros(len(flat), _GRAD_ROW)
-    rows["grad"], rows["n"], rows["dtype"] = list(map(_ptr, flat)), [g.numel() for g in flat], [_lib.DTYPES[g.dtype] for g in flat]
-    lib, at = _lib.load(), _address(rows)
-    with _on(dev):
-        stream = _lib.stream_ptr(dev)
-        ws = torch.empty(2 + lib.rfx_grad_norm_workspace_bytes(at, len(rows)) // 8, dtype=torch.float64, device=dev)
+    lib, rows, n, kind = _lib.load(), _grad_rows(flat), len(flat), 2 if norm_type == 2.0 else 0
+    with _on(index):
+        stream = _lib.stream_ptr(index)
+        ws_bytes = lib.rfx_grad_norm_workspace_bytes(rows, n)
+        ws = torch.empty(2 + ws_bytes // 8, dtype=torch.float64, device=dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
         clip = ws.data_ptr()
-        _lib.check(lib.rfx_grad_norm(at, len(rows), 2 if norm_type == 2.0 else 0, max_norm, clip, norm.data_ptr(), clip + 16,
-                                     ws.numel() * 8 - 16, stream), "rfx_grad_norm")
-        if error_if_nonfinite and not bool(torch.isfinite(norm)):
-            raise RuntimeError(f"the norm of the gradients is not finite ({float(norm)}), so they cannot be clipped")
-        _lib.check(lib.rfx_grad_scale(at, len(rows), clip, stream), "rfx_grad_scale")
-        for g, f in zip(grads, flat):
-            if f is not g:
-                g.copy_(f)
+        if not error_if_nonfinite:
+            _lib.check(lib.rfx_grad_clip(rows, n, kind, max_norm, clip, norm.data_ptr(), clip + 16, ws_bytes, stream), "rfx_grad_clip")
+        else:
+            _lib.check(lib.rfx_grad_norm(rows, n, kind, max_norm, clip, norm.data_ptr(), clip + 16, ws_bytes, stream), "rfx_grad_norm")
+            if not bool(torch.isfinite(norm)):
+                raise RuntimeError(f"the norm of the gradients is not finite ({float(norm)}), so they cannot be clipped")
+            _lib.check(lib.rfx_grad_scale(rows, n, clip, stream), "rfx_grad_scale")
+        if flat is not grads:
+            for g, f in zip(grads, flat):
+                if f is not g:
+                    g.copy_(f)
     return norm
 
 
 class _Plan:
     """what the descriptors of one step hold that stays the same from step to step: the parameters that have a gradient, on one
     device, with their state.  Checked against the optimizer at every step and built again when anything of it changed."""
-    __slots__ = ("device", "params", "ptrs", "shapes", "strides", "dtypes", "states", "parts", "rows", "at", "grads", "grads_at",
-                 "ws_bytes", "index", "spans", "settings", "groups", "flat", "counted", "ordered")
+    __slots__ = ("device", "params", "ptrs", "shapes", "strides", "dtypes", "states", "parts", "flat", "rows", "elems", "grads", "grad_elems",
+                 "ws_bytes", "index", "spans", "settings", "groups", "counted", "ordered", "uniform")
 
 
 class AdamW(torch.optim.AdamW):
@@ -279,7 +291,11 @@ class AdamW(torch.optim.AdamW):
         self.grad_norm = None
 
     _patch_step_function = Adam._patch_step_function
-    _hooked = Adam._hooked
+
+    def _hooked(self):
+        o = _torch_optimizer
+        return bool(self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks
+                    or o._global_optimizer_pre_hooks or o._global_optimizer_post_hooks)
 
     @property
     def max_grad_norm(self):
@@ -397,26 +413,40 @@ class AdamW(torch.optim.AdamW):
     def moments(self):
         """(exp_avg, exp_avg_sq) of all parameters, in their order, as fp32 tensors: the state's own tensors where moments are held
         in 32 bits, the values of the codes where in 8, zeros where there is no state yet"""
-        avg, avg_sq, decode = [], [], {}
+        avg, avg_sq, eight = [], [], {}
         for g in self.param_groups:
             for p in g["params"]:
                 st = self.state.get(p)
                 if not st:
                     avg.append(torch.zeros_like(p, dtype=torch.float32))
                     avg_sq.append(torch.zeros_like(p, dtype=torch.float32))
-                elif st["exp_avg"].dtype != torch.uint8:
+                elif st["exp_avg"].dtype is not torch.uint8:
                     avg.append(st["exp_avg"])
                     avg_sq.append(st["exp_avg_sq"])
                 else:
+                    eight.setdefault(p.device, []).append((len(avg), p, g, st))
+                    avg.append(None)
+                    avg_sq.append(None)
+        for dev, some in eight.items():
+            for _, p, g, st in some:
+                if not (st["exp_avg"].is_contiguous() and st["exp_avg_sq"].is_contiguous() and st["exponents"].numel() == 2 * -(-p.numel() // _lib.ADAMW_BLOCK)
+                        and st["exp_avg"].numel() == st["exp_avg_sq"].numel() == p.numel()):
                     self._check_state(p, g)
-                    m, v = st["exp_avg"], st["exp_avg_sq"]
-                    avg.append(torch.empty_like(m, dtype=torch.float32))
-                    avg_sq.append(torch.empty_like(v, dtype=torch.float32))
-                    decode.setdefault(p.device, []).append(_lib.MomentTensor(m.data_ptr(), v.data_ptr(), st["exponents"].data_ptr(),
-                                                                             avg[-1].data_ptr(), avg_sq[-1].data_ptr(), m.numel()))
-        for dev, ts in decode.items():
-            with _on(dev):
-                _lib.check(_lib.load().rfx_adamw_moments((_lib.MomentTensor * len(ts))(*ts), len(ts), _lib.stream_ptr(dev)), "rfx_adamw_moments")
+            codes = [st["exp_avg"] for _, _, _, st in some]
+            sizes = list(map(_numel, codes))
+            room, total = [], 0                                  # every output at a multiple of 16 bytes
+            for n in sizes:
+                room.append(total)
+                total += (n + 3) & ~3
+            flat = torch.empty(2 * total, dtype=torch.float32, device=dev)
+            at, rows = flat.data_ptr(), []
+            for (i, p, g, st), n, o in zip(some, sizes, room):
+                m = st["exp_avg"]
+                avg[i] = flat.as_strided(m.shape, m.stride(), o)
+                avg_sq[i] = flat.as_strided(m.shape, m.stride(), total + o)
+                rows += (m.data_ptr(), st["exp_avg_sq"].data_ptr(), st["exponents"].data_ptr(), at + 4 * o, at + 4 * (total + o), n)
+            with _on(dev.index):
+                _lib.check(_lib.load().rfx_adamw_moments(struct.pack("QQQQQq" * len(some), *rows), len(some), _lib.stream_ptr(dev)), "rfx_adamw_moments")
         return avg, avg_sq
 
     # ---- the step ---------------------------------------------------------------------------------------------------------
@@ -469,38 +499,40 @@ class AdamW(torch.optim.AdamW):
 
     def _plan(self, dev, part):
         q = _Plan()
+        n = len(part)
         q.device = dev
         q.params = [p for p, _, _ in part]
-        q.index = np.array([i for _, i, _ in part])
+        q.index = [i for _, i, _ in part]
         q.states = [self.state[p] for p in q.params]
         q.parts = [x for st in q.states for x in st.values()]
         q.ptrs, q.flat = list(map(_ptr, q.params)), list(map(_ptr, q.parts))
         q.shapes, q.dtypes = list(map(_size, q.params)), [p.dtype for p in q.params]
         q.strides = list(map(_stride, q.params))
         q.ordered = all(p.stride() == st["exp_avg"].stride() for p, st in zip(q.params, q.states))
-        q.grads = np.zeros(len(part), _GRAD_ROW)
-        q.grads["n"] = [p.numel() for p in q.params]
-        q.grads["dtype"] = [_lib.DTYPES[t] for t in q.dtypes]
-        q.grads_at = _address(q.grads)
+        q.rows, q.grads = (_lib.AdamwTensor * n)(), (_lib.GradTensor * n)()
+        q.elems, q.grad_elems = list(q.rows), list(q.grads)
         q.ws_bytes = None
-        q.rows = np.zeros(len(part), _TENSOR_ROW)
-        q.at = _address(q.rows)
         q.spans, q.settings, q.counted = [], [], False
         for k, (p, i, gi) in enumerate(part):
-            g, st, r = self.param_groups[gi], q.states[k], q.rows[k]
+            g, st, r = self.param_groups[gi], q.states[k], q.elems[k]
             if not q.spans or q.spans[-1][0] != gi:
-                q.spans.append([gi, k, k])
+                q.spans.append([gi, k, k, None])
                 q.settings.append((g["state_bits"], g["master_weights"], g["capturable"]))
             q.spans[-1][2] = k + 1
-            r["param"], r["exp_avg"], r["exp_avg_sq"] = q.ptrs[k], st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()
+            r.param, r.exp_avg, r.exp_avg_sq = q.ptrs[k], st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()
             if g["state_bits"] == 8:
-                r["exponents"] = st["exponents"].data_ptr()
+                r.exponents = st["exponents"].data_ptr()
             if g["master_weights"] and p.dtype != torch.float32:
-                r["master"] = st["master"].data_ptr()
+                r.master = st["master"].data_ptr()
             if g["capturable"]:
-                r["step_dev"], q.counted = st["step"].data_ptr(), True
-            r["n"], r["group"], r["index"], r["dtype"] = p.numel(), len(q.spans) - 1, i, _lib.DTYPES[p.dtype]
-        q.groups = (_lib.AdamwGroup * len(q.spans))()
+                r.step_dev, q.counted = st["step"].data_ptr(), True
+            r.n, r.group, r.index, r.dtype = p.numel(), len(q.spans) - 1, i, _lib.DTYPES[p.dtype]
+            q.grad_elems[k].n, q.grad_elems[k].dtype = r.n, r.dtype
+        for span in q.spans:                                     # the host's step counts of a span: neighbours, or gathered one by one
+            at = q.index[span[1]:span[2]]
+            if at[-1] - at[0] + 1 == len(at) and self._steps is not None:
+                span[3] = self._steps[0][at[0]:at[-1] + 1]
+        q.groups, q.uniform = (_lib.AdamwGroup * len(q.spans))(), True
         return q
 
     def _holds(self, q):
@@ -509,7 +541,7 @@ class AdamW(torch.optim.AdamW):
         return (len(parts) == len(q.parts) and all(map(is_, parts, q.parts)) and list(map(_ptr, parts)) == q.flat
                 and list(map(_ptr, q.params)) == q.ptrs and list(map(_stride, q.params)) == q.strides
                 and list(map(_size, q.params)) == q.shapes and [p.dtype for p in q.params] == q.dtypes
-                and [self._settings(gi) for gi, _, _ in q.spans] == q.settings)
+                and [self._settings(gi) for gi, _, _, _ in q.spans] == q.settings)
 
     def _settings(self, gi):
         g = self.param_groups[gi]
@@ -522,29 +554,41 @@ class AdamW(torch.optim.AdamW):
         self._optimizer_step_code()
         return out
 
-    @torch.no_grad()
     def _step_impl(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        params = [p for g in self.param_groups for p in g["params"] if p.grad is not None]
+        params, grads = [], []
+        for g in self.param_groups:
+            for p in g["params"]:
+                grad = p.grad
+                if grad is not None:
+                    params.append(p)
+                    grads.append(grad)
         if not params:
             return loss
         if not params[0].is_cuda:
             self._cpu_step(params)
             return loss
-        if not self._plans or len(params) != len(self._order) or not all(map(is_, params, self._order)) \
+        plans = self._plans
+        if not plans or len(params) != len(self._order) or not all(map(is_, params, self._order)) \
                 or len(self.state) != len(self._values) or not all(map(is_, self.state.values(), self._values)) \
-                or not all(map(self._holds, self._plans.values())):
+                or not all(map(self._holds, plans.values())):
             if not all(p.is_cuda for p in params):
                 raise _lib.RfxError("parameters on the CPU and on a device in one optimizer are not supported")
-            self._build([(p, i, gi) for i, (gi, p) in enumerate((gi, p) for gi, g in enumerate(self.param_groups) for p in g["params"])
-                         if p.grad is not None])
-        if self.max_grad_norm is not None and len(self._plans) > 1:
-            raise _lib.RfxError("max_grad_norm needs all parameters on one device")
-        for q in self._plans.values():
-            self._launch(q)
+            with torch.no_grad():
+                self._build([(p, i, gi) for i, (gi, p) in enumerate((gi, p) for gi, g in enumerate(self.param_groups) for p in g["params"])
+                             if p.grad is not None])
+            plans = self._plans
+        if len(plans) == 1:
+            for q in plans.values():
+                self._launch(q, grads)
+        else:
+            if self.max_grad_norm is not None:
+                raise _lib.RfxError("max_grad_norm needs all parameters on one device")
+            for q in plans.values():
+                self._launch(q, [p.grad for p in q.params])
         return loss
 
     def _cpu_step(self, params):
@@ -553,51 +597,57 @@ class AdamW(torch.optim.AdamW):
         if self.max_grad_norm is not None or any(g["state_bits"] != 32 or g["master_weights"] for g in self.param_groups):
             raise _lib.RfxError("8-bit moments, master weights and max_grad_norm need device parameters: there is no CPU path")
         torch_step = torch.optim.AdamW.step
-        getattr(torch_step, "__wrapped__", torch_step)(self, None)
+        with torch.no_grad():
+            getattr(torch_step, "__wrapped__", torch_step)(self, None)
 
-    def _launch(self, q):
-        lib, dev = _lib.load(), q.device
-        grads = [p.grad for p in q.params]
+    def _launch(self, q, grads):
+        lib, index, limit = _lib.load(), q.device.index, self.defaults["max_grad_norm"]
         late = None
-        rows, at, grows, grads_at = q.rows, q.at, q.grads, q.grads_at
+        rows, elems, n = q.rows, q.elems, len(grads)
         try:
-            direct = q.ordered and list(map(_stride, grads)) == q.strides and list(map(_size, grads)) == q.shapes and [g.dtype for g in grads] == q.dtypes
-        except RuntimeError:                                   # a layout without strides
+            direct = q.ordered and list(map(_stride, grads)) == q.strides and list(map(_size, grads)) == q.shapes \
+                and [g.dtype for g in grads] == q.dtypes and min(map(_get_device, grads)) == max(map(_get_device, grads)) == index
+        except RuntimeError:                                     # a layout without strides
             direct = False
-        if not direct:
-            rows, grows = rows.copy(), grows.copy()
-            at, grads_at = _address(rows), _address(grows)
-            grads, late = self._in_order(q, grads, rows)
-        grows["grad"] = rows["grad"] = list(map(_ptr, grads))
-        with _on(dev):
-            if not q.counted or any(not s[2] for s in q.settings):
-                if torch.cuda.is_current_stream_capturing():
-                    raise _lib.RfxError("a step without capturable=True cannot be captured: its step count would stand still")
-            groups = self._fill(q, rows)
-            stream = _lib.stream_ptr(dev)
+        with _on(index):
+            if _capturing() and not all(s[2] for s in q.settings):
+                raise _lib.RfxError("a step without capturable=True cannot be captured: its step count would stand still")
+            if not direct:
+                rows = (_lib.AdamwTensor * n).from_buffer_copy(q.rows)
+                elems = list(rows)
+                with torch.no_grad():
+                    grads, late = self._in_order(q, grads, elems)
+            at = list(map(_ptr, grads))
+            for e, a in zip(elems, at):
+                e.grad = a
+            groups = self._fill(q, elems)
+            stream = _lib.stream_ptr(index)
             clip = ws = None
-            if self.max_grad_norm is not None:
+            if limit is not None:
+                for e, a in zip(q.grad_elems, at):
+                    e.grad = a
                 if q.ws_bytes is None:
-                    q.ws_bytes = lib.rfx_grad_norm_workspace_bytes(grads_at, len(grads))
-                buf = torch.empty(2 + q.ws_bytes // 8, dtype=torch.float64, device=dev)
-                self.grad_norm = torch.empty((), dtype=torch.float32, device=dev)
+                    q.ws_bytes = lib.rfx_grad_norm_workspace_bytes(q.grads, n)
+                buf = torch.empty(2 + q.ws_bytes // 8, dtype=torch.float64, device=q.device)
+                self.grad_norm = torch.empty((), dtype=torch.float32, device=q.device)
                 clip = buf.data_ptr()
-                _lib.check(lib.rfx_grad_norm(grads_at, len(grads), 2, self.max_grad_norm, clip, self.grad_norm.data_ptr(), clip + 16,
-                                             q.ws_bytes, stream), "rfx_grad_norm")
+                _lib.check(lib.rfx_grad_norm(q.grads, n, 2, limit, clip, self.grad_norm.data_ptr(), clip + 16, q.ws_bytes, stream),
+                           "rfx_grad_norm")
             n_ws = 0
             if q.counted:
-                n_ws = lib.rfx_adamw_workspace_bytes(len(grads))
-                ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
-            _lib.check(lib.rfx_adamw_step(at, len(grads), groups, len(groups), clip, None if ws is None else ws.data_ptr(), n_ws, stream),
+                n_ws = lib.rfx_adamw_workspace_bytes(n)
+                ws = torch.empty(n_ws, dtype=torch.uint8, device=q.device)
+            _lib.check(lib.rfx_adamw_step(rows, n, groups, len(groups), clip, None if ws is None else ws.data_ptr(), n_ws, stream),
                        "rfx_adamw_step")
             if late:
-                for p, x in late:
-                    p.copy_(x)
+                with torch.no_grad():
+                    for p, x in late:
+                        p.copy_(x)
 
-    def _in_order(self, q, grads, rows):
+    def _in_order(self, q, grads, elems):
         """gradients (and parameters with gaps) brought to the memory order of their moments; `late`: what goes back afterwards"""
         out, late = [], []
-        for k, (p, g, st) in enumerate(zip(q.params, grads, q.states)):
+        for p, g, st, e in zip(q.params, grads, q.states, elems):
             _check_grad(g)
             if g.dtype != p.dtype or g.shape != p.shape or g.device != p.device:
                 raise _lib.RfxError(f"a gradient of type {g.dtype}, shape {tuple(g.shape)} on {g.device} for a parameter of type {p.dtype}, "
@@ -606,14 +656,14 @@ class AdamW(torch.optim.AdamW):
             if not _same_memory_order(p, m):
                 x = torch.empty_like(m, dtype=p.dtype).copy_(p)
                 late.append((p, x))
-                rows[k]["param"] = x.data_ptr()
+                e.param = x.data_ptr()
             out.append(g if _same_memory_order(g, m) else torch.empty_like(m, dtype=g.dtype).copy_(g))
         return out, late
 
-    def _fill(self, q, rows):
+    def _fill(self, q, elems):
         """raises the host's step counts and writes what belongs to a parameter group; more entries where its counts differ"""
-        groups, n = q.groups, len(q.spans)
-        for k, (gi, lo, hi) in enumerate(q.spans):
+        groups, even = q.groups, True
+        for k, (gi, lo, hi, counts) in enumerate(q.spans):
             g, e = self.param_groups[gi], groups[k]
             lr = g["lr"]
             if isinstance(lr, torch.Tensor):
@@ -626,19 +676,28 @@ class AdamW(torch.optim.AdamW):
             e.eps, e.weight_decay, e.seed, e.state_bits, e.maximize = g["eps"], g["weight_decay"], g["seed"], g["state_bits"], g["maximize"]
             if g["capturable"]:
                 continue
-            steps = self._steps[0]
-            at = q.index[lo:hi]
-            now = steps[at] + 1.0
-            steps[at] = now
-            e.step = int(now[0])
-            if not (now == now[0]).all():                      # parameters that joined at different steps
-                counts = sorted({int(x) for x in now})
-                more = (_lib.AdamwGroup * (len(groups) + len(counts)))(*groups)
-                for j, c in enumerate(counts):
-                    more[len(groups) + j] = e
-                    more[len(groups) + j].step = c
-                    rows["group"][lo:hi][now == c] = len(groups) + j
-                groups = more
+            if counts is not None:
+                counts += 1.0
+                now = counts.tolist()
             else:
-                rows["group"][lo:hi] = k
+                steps = self._steps[0]
+                now = [float(steps[i]) + 1.0 for i in q.index[lo:hi]]
+                steps[q.index[lo:hi]] = now
+            e.step = int(now[0])
+            if now.count(now[0]) == len(now):
+                if not q.uniform or elems is not q.elems:
+                    for r in elems[lo:hi]:
+                        r.group = k
+                continue
+            even = False                                         # parameters that joined at different steps
+            first = len(groups)
+            kinds = sorted(set(now))
+            more = (_lib.AdamwGroup * (first + len(kinds)))(*groups)
+            for j, c in enumerate(kinds):
+                more[first + j] = e
+                more[first + j].step = int(c)
+            for r, c in zip(elems[lo:hi], now):
+                r.group = first + kinds.index(c)
+            groups = more
+        q.uniform = even
         return groups
