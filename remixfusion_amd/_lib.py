@@ -276,6 +276,24 @@ def load() -> C.CDLL:
     return lib
 
 
+_host = None
+
+
+def host():
+    """the optimizers' host module (csrc/optim_host.cpp), bound to librfx's entry points"""
+    global _host
+    if _host is None:
+        lib = load()
+        try:
+            from . import _optim_host
+        except ImportError as e:
+            raise RfxError(f"_optim_host.so cannot be loaded ({e}): build it with `python -m remixfusion_amd.build`") from e
+        _optim_host.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in (
+            "rfx_adamw_step", "rfx_adamw_workspace_bytes", "rfx_adamw_moments", "rfx_grad_norm_workspace_bytes", "rfx_grad_norm", "rfx_grad_clip")})
+        _host = _optim_host
+    return _host
+
+
 def check(status: int, what: str) -> None:
     if status != 0:
         extra = f" (hipError {load().rfx_last_hip_error()})" if status == -2 else ""

@@ -33,6 +33,34 @@ def _hipcc() -> str:
     raise RuntimeError("hipcc not found: librfx.so cannot be built (no CPU fallback exists)")
 
 
+HOST_LIB = os.path.join(HERE, "_optim_host.so")
+HOST_SOURCE = os.path.join(CSRC, "optim_host.cpp")
+
+
+def build_host(force: bool = False, verbose: bool = False) -> str:
+    """_optim_host.so: the CPython module of the optimizers' host side (host code only, g++ against torch's headers)."""
+    deps = [HOST_SOURCE, os.path.abspath(os.path.join(CSRC, "..", "..", "include", "rfx.h")), os.path.abspath(__file__)]
+    if not force and os.path.exists(HOST_LIB) and all(os.path.getmtime(d) <= os.path.getmtime(HOST_LIB) for d in deps if os.path.exists(d)):
+        return HOST_LIB
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    inc = [f"-I{d}" for d in cpp_extension.include_paths() + [sysconfig.get_paths()["include"]]]
+    cmd = ([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + inc
+           + ["-o", HOST_LIB + ".tmp", HOST_SOURCE, f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{lib}"])
+    if verbose:
+        print(" ".join(cmd))
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("g++ failed building _optim_host.so")
+    os.replace(HOST_LIB + ".tmp", HOST_LIB)
+    return HOST_LIB
+
+
 def _stale() -> bool:
     if not os.path.exists(LIB):
         return True
@@ -84,3 +112,4 @@ def build_library(force: bool = False, verbose: bool = False, extra: List[str] |
 
 if __name__ == "__main__":
     print(build_library(force="--force" in sys.argv, verbose=True))
+    print(build_host(force="--force" in sys.argv, verbose=True))

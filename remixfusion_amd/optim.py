@@ -9,8 +9,6 @@ maximize, closures that need grad mode) takes torch's own implementation.
 """
 import ctypes as C
 import math
-import struct
-from operator import is_
 
 import torch
 from torch.optim import optimizer as _torch_optimizer
@@ -138,10 +136,7 @@ class Adam(torch.optim.Adam):
         return loss
 
 
-_size, _stride, _ptr, _numel, _get_device = (getattr(torch.Tensor, k) for k in ("size", "stride", "data_ptr", "numel", "get_device"))
-_is_contiguous = torch.Tensor.is_contiguous
 _capturing = torch._C._cuda_isCurrentStreamCapturing if hasattr(torch._C, "_cuda_isCurrentStreamCapturing") else (lambda: False)
-_TYPE_OF = _lib.DTYPES.get
 
 
 def _same_memory_order(a, b):
@@ -192,8 +187,7 @@ def _check_grad(g):
 
 def _grad_rows(grads):
     """rfx_grad_tensor descriptors of gradients of the known types"""
-    rows = [x for row in zip(map(_ptr, grads), map(_numel, grads), [_TYPE_OF(g.dtype) for g in grads]) for x in row]
-    return struct.pack("Qqi4x" * len(grads), *rows)
+    return (_lib.GradTensor * len(grads))(*[_lib.GradTensor(g.data_ptr(), g.numel(), _lib.DTYPES[g.dtype], 0) for g in grads])
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -204,54 +198,44 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     not finite is applied as it is: an infinite norm makes zeros (and NaN of what was infinite), a NaN makes NaN.  One device;
     float32 / bfloat16 / float16 gradients, mixed freely.  Gradients on the CPU take torch's own function."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    grads = [p.grad for p in parameters if p.grad is not None]
     max_norm, norm_type = float(max_norm), float(norm_type)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm has to be a number >= 0: {max_norm}")
+    if parameters and parameters[0].is_cuda and not error_if_nonfinite and norm_type in (2.0, math.inf):
+        index = torch._C._cuda_getDevice()
+        out = _lib.host().clip(parameters, 2 if norm_type == 2.0 else 0, max_norm, index, _lib.stream_ptr(index))
+        if isinstance(out, torch.Tensor):
+            return out
+        _lib.check(min(out, 0), "rfx_grad_clip")
+    # what is left: no gradient, another device than the current one, gradients with gaps in memory, types and layouts to be refused
+    grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.tensor(0.0)
-    index = max(map(_get_device, grads))
-    if index < 0:
+    if not any(g.is_cuda for g in grads):
         return torch.nn.utils.clip_grad_norm_(parameters, max_norm, norm_type, error_if_nonfinite)
     if norm_type not in (2.0, math.inf):
         raise _lib.RfxError(f"norm_type {norm_type}: only 2 and inf are supported")
-    if any(g.layout is not torch.strided or g.dtype not in _lib.DTYPES for g in grads):
-        for g in grads:
-            _check_grad(g)
-    if min(map(_get_device, grads)) != index:
-        raise _lib.RfxError("gradients on different devices: clip them device by device")
-    flat = grads
-    if not all(map(_is_contiguous, grads)):
-        for g in grads:
-            _check_grad(g)
-        flat = [g if _dense(g) else g.contiguous() for g in grads]
     dev = grads[0].device
+    for g in grads:
+        _check_grad(g)
+        if g.device != dev:
+            raise _lib.RfxError("gradients on different devices: clip them device by device")
+    flat = [g if _dense(g) else g.contiguous() for g in grads]
     lib, rows, n, kind = _lib.load(), _grad_rows(flat), len(flat), 2 if norm_type == 2.0 else 0
-    with _on(index):
-        stream = _lib.stream_ptr(index)
+    with _on(dev.index), torch.no_grad():
+        stream = _lib.stream_ptr(dev)
         ws_bytes = lib.rfx_grad_norm_workspace_bytes(rows, n)
         ws = torch.empty(2 + ws_bytes // 8, dtype=torch.float64, device=dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
         clip = ws.data_ptr()
-        if not error_if_nonfinite:
-            _lib.check(lib.rfx_grad_clip(rows, n, kind, max_norm, clip, norm.data_ptr(), clip + 16, ws_bytes, stream), "rfx_grad_clip")
-        else:
-            _lib.check(lib.rfx_grad_norm(rows, n, kind, max_norm, clip, norm.data_ptr(), clip + 16, ws_bytes, stream), "rfx_grad_norm")
-            if not bool(torch.isfinite(norm)):
-                raise RuntimeError(f"the norm of the gradients is not finite ({float(norm)}), so they cannot be clipped")
-            _lib.check(lib.rfx_grad_scale(rows, n, clip, stream), "rfx_grad_scale")
-        if flat is not grads:
-            for g, f in zip(grads, flat):
-                if f is not g:
-                    g.copy_(f)
+        _lib.check(lib.rfx_grad_norm(rows, n, kind, max_norm, clip, norm.data_ptr(), clip + 16, ws_bytes, stream), "rfx_grad_norm")
+        if error_if_nonfinite and not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"the norm of the gradients is not finite ({float(norm)}), so they cannot be clipped")
+        _lib.check(lib.rfx_grad_scale(rows, n, clip, stream), "rfx_grad_scale")
+        for g, f in zip(grads, flat):
+            if f is not g:
+                g.copy_(f)
     return norm
-
-
-class _Plan:
-    """what the descriptors of one step hold that stays the same from step to step: the parameters that have a gradient, on one
-    device, with their state.  Checked against the optimizer at every step and built again when anything of it changed."""
-    __slots__ = ("device", "params", "ptrs", "shapes", "strides", "dtypes", "states", "parts", "flat", "rows", "elems", "grads", "grad_elems",
-                 "ws_bytes", "index", "spans", "settings", "groups", "counted", "ordered", "uniform")
 
 
 class AdamW(torch.optim.AdamW):
@@ -287,8 +271,7 @@ class AdamW(torch.optim.AdamW):
         self.defaults.update(self._own, max_grad_norm=None if max_grad_norm is None else float(max_grad_norm))
 
     def _reset(self):
-        self._plans, self._steps, self._dev_steps = {}, None, {}
-        self.grad_norm = None
+        self._plans, self.grad_norm = {}, None
 
     _patch_step_function = Adam._patch_step_function
 
@@ -381,6 +364,11 @@ class AdamW(torch.optim.AdamW):
             if e.dtype != torch.int8 or tuple(e.shape) != (2, -(-p.numel() // _lib.ADAMW_BLOCK)) or e.device != p.device:
                 raise _lib.RfxError(f"exponents of type {e.dtype}, shape {tuple(e.shape)} on {e.device}: int8 [2, {-(-p.numel() // _lib.ADAMW_BLOCK)}] is needed")
             st["exponents"] = e.contiguous()
+        step, at = st["step"], p.device if g["capturable"] else torch.device("cpu")
+        if not isinstance(step, torch.Tensor) or step.device != at or step.dtype != torch.float32 or step.numel() != 1:
+            if torch.cuda.is_current_stream_capturing():
+                raise _lib.RfxError("the step count is not where a captured step needs it: call step() or prepare() before capturing")
+            st["step"] = torch.as_tensor(step, dtype=torch.float32).detach().reshape(()).to(at)
         if g["master_weights"] and p.dtype != torch.float32:
             w = st.get("master")
             if w is None or tuple(w.shape) != tuple(p.shape) or w.dtype != torch.float32 or w.device != p.device or not (
@@ -391,7 +379,7 @@ class AdamW(torch.optim.AdamW):
 
     def _new_state(self, p, g):
         st = self.state[p]
-        st["step"] = torch.tensor(0.0, dtype=torch.float32)
+        st["step"] = torch.zeros((), dtype=torch.float32, device=p.device if g["capturable"] else "cpu")
         kind = torch.uint8 if g["state_bits"] == 8 else torch.float32
         st["exp_avg"] = torch.zeros_like(p, dtype=kind, memory_format=torch.preserve_format)
         st["exp_avg_sq"] = torch.zeros_like(st["exp_avg"])
@@ -409,7 +397,6 @@ class AdamW(torch.optim.AdamW):
         if every:
             self._build(every)
 
-    @torch.no_grad()
     def moments(self):
         """(exp_avg, exp_avg_sq) of all parameters, in their order, as fp32 tensors: the state's own tensors where moments are held
         in 32 bits, the values of the codes where in 8, zeros where there is no state yet"""
@@ -417,135 +404,48 @@ class AdamW(torch.optim.AdamW):
         for g in self.param_groups:
             for p in g["params"]:
                 st = self.state.get(p)
-                if not st:
-                    avg.append(torch.zeros_like(p, dtype=torch.float32))
-                    avg_sq.append(torch.zeros_like(p, dtype=torch.float32))
-                elif st["exp_avg"].dtype is not torch.uint8:
-                    avg.append(st["exp_avg"])
-                    avg_sq.append(st["exp_avg_sq"])
+                if st and st["exp_avg"].dtype is torch.uint8:
+                    at, states = eight.setdefault(st["exp_avg"].get_device(), ([], []))
+                    at.append(len(avg))
+                    states.append(st)
+                    m = v = None
+                elif st:
+                    m, v = st["exp_avg"], st["exp_avg_sq"]
                 else:
-                    eight.setdefault(p.device, []).append((len(avg), p, g, st))
-                    avg.append(None)
-                    avg_sq.append(None)
-        for dev, some in eight.items():
-            for _, p, g, st in some:
-                if not (st["exp_avg"].is_contiguous() and st["exp_avg_sq"].is_contiguous() and st["exponents"].numel() == 2 * -(-p.numel() // _lib.ADAMW_BLOCK)
-                        and st["exp_avg"].numel() == st["exp_avg_sq"].numel() == p.numel()):
-                    self._check_state(p, g)
-            codes = [st["exp_avg"] for _, _, _, st in some]
-            sizes = list(map(_numel, codes))
-            room, total = [], 0                                  # every output at a multiple of 16 bytes
-            for n in sizes:
-                room.append(total)
-                total += (n + 3) & ~3
-            flat = torch.empty(2 * total, dtype=torch.float32, device=dev)
-            at, rows = flat.data_ptr(), []
-            for (i, p, g, st), n, o in zip(some, sizes, room):
-                m = st["exp_avg"]
-                avg[i] = flat.as_strided(m.shape, m.stride(), o)
-                avg_sq[i] = flat.as_strided(m.shape, m.stride(), total + o)
-                rows += (m.data_ptr(), st["exp_avg_sq"].data_ptr(), st["exponents"].data_ptr(), at + 4 * o, at + 4 * (total + o), n)
-            with _on(dev.index):
-                _lib.check(_lib.load().rfx_adamw_moments(struct.pack("QQQQQq" * len(some), *rows), len(some), _lib.stream_ptr(dev)), "rfx_adamw_moments")
+                    m, v = (torch.zeros_like(p, dtype=torch.float32, requires_grad=False) for _ in range(2))
+                avg.append(m)
+                avg_sq.append(v)
+        for index, (at, states) in eight.items():
+            with _on(index):
+                out = _lib.host().moments(states, _lib.stream_ptr(index))
+            if isinstance(out, int):
+                _lib.check(out, "rfx_adamw_moments")
+            for i, m, v in zip(at, *out):
+                avg[i], avg_sq[i] = m, v
         return avg, avg_sq
 
     # ---- the step ---------------------------------------------------------------------------------------------------------
-    def _counters(self, n):
-        """the step counts of all parameters as one host array; state[p]["step"] is its element's view"""
-        if self._steps is None or len(self._steps[0]) != n:
-            t = torch.zeros(n, dtype=torch.float32)
-            self._steps = (t.numpy(), list(t))
-        return self._steps
-
     def _build(self, every):
         """plans for (parameter, its place in the optimizer, its group): states made or checked, one plan per device"""
         capturing = torch.cuda.is_current_stream_capturing()
-        total = sum(len(g["params"]) for g in self.param_groups)
-        _, views = self._counters(total)
         by_device = {}
-        for p, i, gi in every:
-            by_device.setdefault(p.device, []).append((p, i, gi))
-        for dev, part in by_device.items():
-            for p, i, gi in part:
-                g = self.param_groups[gi]
-                if p.dtype not in _lib.DTYPES:
-                    raise _lib.RfxError(f"parameters of type {p.dtype} are not supported: float32, bfloat16 or float16")
-                if _overlaps_itself(p):
-                    raise _lib.RfxError("a parameter whose elements share memory (an expanded tensor) is not supported")
-                st = self.state.get(p)
-                if not st:
-                    if capturing:
-                        raise _lib.RfxError("the state is created by the first step() or prepare(): call it before capturing")
-                    self._new_state(p, g)
-                else:
-                    self._check_state(p, g)
-                st = self.state[p]
-                if g["capturable"]:
-                    have = self._dev_steps.get(dev)
-                    if have is None or len(have) != total:
-                        if capturing:
-                            raise _lib.RfxError("the state is created by the first step() or prepare(): call it before capturing")
-                        have = self._dev_steps[dev] = list(torch.zeros(total, dtype=torch.float32, device=dev))
-                    view = have[i]
-                else:
-                    view = views[i]
-                if st["step"] is not view:
-                    if capturing:
-                        raise _lib.RfxError("the state is created by the first step() or prepare(): call it before capturing")
-                    view.copy_(st["step"].detach().reshape(()))
-                    st["step"] = view
-        self._plans = {dev: self._plan(dev, part) for dev, part in by_device.items()}
-        self._order, self._values = [p for p, _, _ in every], list(self.state.values())
-
-    def _plan(self, dev, part):
-        q = _Plan()
-        n = len(part)
-        q.device = dev
-        q.params = [p for p, _, _ in part]
-        q.index = [i for _, i, _ in part]
-        q.states = [self.state[p] for p in q.params]
-        q.parts = [x for st in q.states for x in st.values()]
-        q.ptrs, q.flat = list(map(_ptr, q.params)), list(map(_ptr, q.parts))
-        q.shapes, q.dtypes = list(map(_size, q.params)), [p.dtype for p in q.params]
-        q.strides = list(map(_stride, q.params))
-        q.ordered = all(p.stride() == st["exp_avg"].stride() for p, st in zip(q.params, q.states))
-        q.rows, q.grads = (_lib.AdamwTensor * n)(), (_lib.GradTensor * n)()
-        q.elems, q.grad_elems = list(q.rows), list(q.grads)
-        q.ws_bytes = None
-        q.spans, q.settings, q.counted = [], [], False
-        for k, (p, i, gi) in enumerate(part):
-            g, st, r = self.param_groups[gi], q.states[k], q.elems[k]
-            if not q.spans or q.spans[-1][0] != gi:
-                q.spans.append([gi, k, k, None])
-                q.settings.append((g["state_bits"], g["master_weights"], g["capturable"]))
-            q.spans[-1][2] = k + 1
-            r.param, r.exp_avg, r.exp_avg_sq = q.ptrs[k], st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()
-            if g["state_bits"] == 8:
-                r.exponents = st["exponents"].data_ptr()
-            if g["master_weights"] and p.dtype != torch.float32:
-                r.master = st["master"].data_ptr()
-            if g["capturable"]:
-                r.step_dev, q.counted = st["step"].data_ptr(), True
-            r.n, r.group, r.index, r.dtype = p.numel(), len(q.spans) - 1, i, _lib.DTYPES[p.dtype]
-            q.grad_elems[k].n, q.grad_elems[k].dtype = r.n, r.dtype
-        for span in q.spans:                                     # the host's step counts of a span: neighbours, or gathered one by one
-            at = q.index[span[1]:span[2]]
-            if at[-1] - at[0] + 1 == len(at) and self._steps is not None:
-                span[3] = self._steps[0][at[0]:at[-1] + 1]
-        q.groups, q.uniform = (_lib.AdamwGroup * len(q.spans))(), True
-        return q
-
-    def _holds(self, q):
-        """whether a plan still says where everything is"""
-        parts = [x for st in q.states for x in st.values()]
-        return (len(parts) == len(q.parts) and all(map(is_, parts, q.parts)) and list(map(_ptr, parts)) == q.flat
-                and list(map(_ptr, q.params)) == q.ptrs and list(map(_stride, q.params)) == q.strides
-                and list(map(_size, q.params)) == q.shapes and [p.dtype for p in q.params] == q.dtypes
-                and [self._settings(gi) for gi, _, _, _ in q.spans] == q.settings)
-
-    def _settings(self, gi):
-        g = self.param_groups[gi]
-        return g["state_bits"], g["master_weights"], g["capturable"]
+        for entry in every:
+            p, _, gi = entry
+            g = self.param_groups[gi]
+            by_device.setdefault(p.device, []).append(entry)
+            if not p.is_cuda:
+                raise _lib.RfxError("parameters on the CPU and on a device in one optimizer are not supported")
+            if p.dtype not in _lib.DTYPES:
+                raise _lib.RfxError(f"parameters of type {p.dtype} are not supported: float32, bfloat16 or float16")
+            if p.layout is not torch.strided or _overlaps_itself(p):
+                raise _lib.RfxError("a parameter whose elements share memory (an expanded tensor) or that is sparse is not supported")
+            if self.state.get(p):
+                self._check_state(p, g)
+            elif capturing:
+                raise _lib.RfxError("the state is created by the first step() or prepare(): call it before capturing")
+            else:
+                self._new_state(p, g)
+        self._plans = {dev: (_lib.host().Plan(part, self.param_groups, self.state), part) for dev, part in by_device.items()}
 
     def step(self, closure=None):
         if self._hooked():
@@ -559,145 +459,66 @@ class AdamW(torch.optim.AdamW):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        params, grads = [], []
-        for g in self.param_groups:
-            for p in g["params"]:
-                grad = p.grad
-                if grad is not None:
-                    params.append(p)
-                    grads.append(grad)
+        limit = self.defaults["max_grad_norm"]
+        other = False
+        if len(self._plans) == 1:
+            for dev, (plan, _) in self._plans.items():
+                with _on(dev.index):
+                    if _capturing() and plan.host_counted:
+                        raise _lib.RfxError("a step without capturable=True cannot be captured: its step count would stand still")
+                    out = plan.step(self.param_groups, self.state, -1.0 if limit is None else limit, _lib.stream_ptr(dev.index))
+                if self._took(out):
+                    return loss
+                other = out == _lib.host().OTHER_ORDER
+        params = [p for g in self.param_groups for p in g["params"] if p.grad is not None]
         if not params:
             return loss
-        if not params[0].is_cuda:
-            self._cpu_step(params)
+        if not any(p.is_cuda for p in params):
+            self._cpu_step()
             return loss
-        plans = self._plans
-        if not plans or len(params) != len(self._order) or not all(map(is_, params, self._order)) \
-                or len(self.state) != len(self._values) or not all(map(is_, self.state.values(), self._values)) \
-                or not all(map(self._holds, plans.values())):
-            if not all(p.is_cuda for p in params):
-                raise _lib.RfxError("parameters on the CPU and on a device in one optimizer are not supported")
-            with torch.no_grad():
+        # nothing planned yet, or something is not as planned; other devices than the current one; gradients in another memory order
+        with torch.no_grad():
+            if not other:
                 self._build([(p, i, gi) for i, (gi, p) in enumerate((gi, p) for gi, g in enumerate(self.param_groups) for p in g["params"])
                              if p.grad is not None])
-            plans = self._plans
-        if len(plans) == 1:
-            for q in plans.values():
-                self._launch(q, grads)
-        else:
-            if self.max_grad_norm is not None:
+            if limit is not None and len(self._plans) > 1:
                 raise _lib.RfxError("max_grad_norm needs all parameters on one device")
-            for q in plans.values():
-                self._launch(q, [p.grad for p in q.params])
+            for dev, (plan, part) in self._plans.items():
+                with _on(dev.index):
+                    if _capturing() and plan.host_counted:
+                        raise _lib.RfxError("a step without capturable=True cannot be captured: its step count would stand still")
+                    stepped, grads = self._in_order([p for p, _, _ in part])
+                    self._took(plan.launch(stepped, grads, self.param_groups, -1.0 if limit is None else limit, _lib.stream_ptr(dev)))
+                    for (p, _, _), x in zip(part, stepped):
+                        if x is not p:
+                            p.copy_(x)
         return loss
 
-    def _cpu_step(self, params):
-        if any(p.is_cuda for p in params):
-            raise _lib.RfxError("parameters on the CPU and on a device in one optimizer are not supported")
+    def _took(self, out):
+        """a plan's answer: the gradients' norm or None, or the number that says why not"""
+        if isinstance(out, int):
+            _lib.check(min(out, 0), "rfx_adamw_step")
+            return False
+        if out is not None:
+            self.grad_norm = out
+        return True
+
+    def _cpu_step(self):
         if self.max_grad_norm is not None or any(g["state_bits"] != 32 or g["master_weights"] for g in self.param_groups):
             raise _lib.RfxError("8-bit moments, master weights and max_grad_norm need device parameters: there is no CPU path")
         torch_step = torch.optim.AdamW.step
         with torch.no_grad():
             getattr(torch_step, "__wrapped__", torch_step)(self, None)
 
-    def _launch(self, q, grads):
-        lib, index, limit = _lib.load(), q.device.index, self.defaults["max_grad_norm"]
-        late = None
-        rows, elems, n = q.rows, q.elems, len(grads)
-        try:
-            direct = q.ordered and list(map(_stride, grads)) == q.strides and list(map(_size, grads)) == q.shapes \
-                and [g.dtype for g in grads] == q.dtypes and min(map(_get_device, grads)) == max(map(_get_device, grads)) == index
-        except RuntimeError:                                     # a layout without strides
-            direct = False
-        with _on(index):
-            if _capturing() and not all(s[2] for s in q.settings):
-                raise _lib.RfxError("a step without capturable=True cannot be captured: its step count would stand still")
-            if not direct:
-                rows = (_lib.AdamwTensor * n).from_buffer_copy(q.rows)
-                elems = list(rows)
-                with torch.no_grad():
-                    grads, late = self._in_order(q, grads, elems)
-            at = list(map(_ptr, grads))
-            for e, a in zip(elems, at):
-                e.grad = a
-            groups = self._fill(q, elems)
-            stream = _lib.stream_ptr(index)
-            clip = ws = None
-            if limit is not None:
-                for e, a in zip(q.grad_elems, at):
-                    e.grad = a
-                if q.ws_bytes is None:
-                    q.ws_bytes = lib.rfx_grad_norm_workspace_bytes(q.grads, n)
-                buf = torch.empty(2 + q.ws_bytes // 8, dtype=torch.float64, device=q.device)
-                self.grad_norm = torch.empty((), dtype=torch.float32, device=q.device)
-                clip = buf.data_ptr()
-                _lib.check(lib.rfx_grad_norm(q.grads, n, 2, limit, clip, self.grad_norm.data_ptr(), clip + 16, q.ws_bytes, stream),
-                           "rfx_grad_norm")
-            n_ws = 0
-            if q.counted:
-                n_ws = lib.rfx_adamw_workspace_bytes(n)
-                ws = torch.empty(n_ws, dtype=torch.uint8, device=q.device)
-            _lib.check(lib.rfx_adamw_step(rows, n, groups, len(groups), clip, None if ws is None else ws.data_ptr(), n_ws, stream),
-                       "rfx_adamw_step")
-            if late:
-                with torch.no_grad():
-                    for p, x in late:
-                        p.copy_(x)
-
-    def _in_order(self, q, grads, elems):
-        """gradients (and parameters with gaps) brought to the memory order of their moments; `late`: what goes back afterwards"""
-        out, late = [], []
-        for p, g, st, e in zip(q.params, grads, q.states, elems):
+    def _in_order(self, params):
+        """parameters and gradients in the memory order of their moments: themselves where they are, copies where not"""
+        stepped, grads = [], []
+        for p in params:
+            g, m = p.grad, self.state[p]["exp_avg"]
             _check_grad(g)
             if g.dtype != p.dtype or g.shape != p.shape or g.device != p.device:
                 raise _lib.RfxError(f"a gradient of type {g.dtype}, shape {tuple(g.shape)} on {g.device} for a parameter of type {p.dtype}, "
                                     f"shape {tuple(p.shape)} on {p.device}")
-            m = st["exp_avg"]
-            if not _same_memory_order(p, m):
-                x = torch.empty_like(m, dtype=p.dtype).copy_(p)
-                late.append((p, x))
-                e.param = x.data_ptr()
-            out.append(g if _same_memory_order(g, m) else torch.empty_like(m, dtype=g.dtype).copy_(g))
-        return out, late
-
-    def _fill(self, q, elems):
-        """raises the host's step counts and writes what belongs to a parameter group; more entries where its counts differ"""
-        groups, even = q.groups, True
-        for k, (gi, lo, hi, counts) in enumerate(q.spans):
-            g, e = self.param_groups[gi], groups[k]
-            lr = g["lr"]
-            if isinstance(lr, torch.Tensor):
-                if not g["capturable"] or not lr.is_cuda or lr.device != q.device or lr.dtype != torch.float32 or lr.numel() != 1:
-                    raise _lib.RfxError("a tensor lr needs capturable=True and has to be one float32 on the parameters' device")
-                e.lr_dev = lr.data_ptr()
-            else:
-                e.lr, e.lr_dev = lr, None
-            e.beta1, e.beta2 = g["betas"]
-            e.eps, e.weight_decay, e.seed, e.state_bits, e.maximize = g["eps"], g["weight_decay"], g["seed"], g["state_bits"], g["maximize"]
-            if g["capturable"]:
-                continue
-            if counts is not None:
-                counts += 1.0
-                now = counts.tolist()
-            else:
-                steps = self._steps[0]
-                now = [float(steps[i]) + 1.0 for i in q.index[lo:hi]]
-                steps[q.index[lo:hi]] = now
-            e.step = int(now[0])
-            if now.count(now[0]) == len(now):
-                if not q.uniform or elems is not q.elems:
-                    for r in elems[lo:hi]:
-                        r.group = k
-                continue
-            even = False                                         # parameters that joined at different steps
-            first = len(groups)
-            kinds = sorted(set(now))
-            more = (_lib.AdamwGroup * (first + len(kinds)))(*groups)
-            for j, c in enumerate(kinds):
-                more[first + j] = e
-                more[first + j].step = int(c)
-            for r, c in zip(elems[lo:hi], now):
-                r.group = first + kinds.index(c)
-            groups = more
-        q.uniform = even
-        return groups
+            stepped.append(p if _same_memory_order(p, m) else torch.empty_like(m, dtype=p.dtype).copy_(p))
+            grads.append(g if _same_memory_order(g, m) else torch.empty_like(m, dtype=g.dtype).copy_(g))
+        return stepped, grads
