@@ -22,7 +22,8 @@ HEADERS = ["rfx_common.h", "rfx_field_device.h", "rfx_field_mlp.h", os.path.join
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     "-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt", "-fno-fast-math",
-    "-Wall", "-Wno-unused-function", "-DHASH_GROUP=4", "-DFWD_WAVES=2", "-DRENDER_WAVES=2", "-DBWD_WAVES=2",
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",      # no v_pk_*_f32: some of their forms are not reliable
+    "-Wall", "-Wno-unused-function", "-Wno-unused-command-line-argument", "-DHASH_GROUP=4", "-DFWD_WAVES=2", "-DRENDER_WAVES=2", "-DBWD_WAVES=2",
 ]
 
 
