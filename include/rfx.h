@@ -767,12 +767,21 @@ typedef struct rfx_adamw_group {
 } rfx_adamw_group;
 size_t rfx_adamw_tensor_bytes(void);
 size_t rfx_adamw_group_bytes(void);
+typedef struct rfx_grad_tensor {
+    void*   grad;                       /* dev [n] */
+    int64_t n;
+    int32_t dtype;
+    int32_t reserved;
+} rfx_grad_tensor;
 /* tensors / groups: host arrays of any length (read before the call returns); few launches for all of them.  Tensors of one
- * call that share parameter memory are stepped one after the other.  clip: dev [2] as rfx_grad_norm writes it, or NULL.
- * workspace: dev, 16-byte aligned, >= rfx_adamw_workspace_bytes(count) where a tensor has step_dev, else NULL.              */
+ * call that share parameter memory are stepped one after the other.  clip_grads: NULL, or the `count` gradients again, whose
+ * 2-norm N is formed first: they enter the moments times min(1, max_norm / (N + 1e-6)) and stay as they are themselves; norm32
+ * (dev [1] or NULL) gets N.  workspace: dev, 16-byte aligned, >= rfx_adamw_workspace_bytes(count) where a tensor has step_dev or
+ * there are clip_grads, else NULL.                                                                                          */
 size_t rfx_adamw_workspace_bytes(int count);
-int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_group* groups, int n_groups, const double* clip,
-                   void* workspace, size_t workspace_bytes, rfx_stream stream);
+int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_group* groups, int n_groups,
+                   const rfx_grad_tensor* clip_grads, double max_norm, float* norm32, void* workspace, size_t workspace_bytes,
+                   rfx_stream stream);
 /* fp32 values of 8-bit moments (what a checkpoint in 32 bits or a look at the state needs), all tensors in few launches. */
 typedef struct rfx_moment_tensor {
     const uint8_t* exp_avg;             /* dev [n], 4-byte aligned */
@@ -786,20 +795,14 @@ int rfx_adamw_moments(const rfx_moment_tensor* tensors, int count, rfx_stream st
 /* Norm of all gradients together and the factor that brings it under max_norm:
  *   norm_type 2: N = sqrt(sum g^2), summed in fp64 in an order that depends on the sizes only; 0: N = max |g| (NaN if one is)
  *   clip[0] = N, clip[1] = min(1, max_norm / (N + 1e-6)); norm32 (or NULL) gets N in fp32.
- * rfx_grad_scale multiplies the gradients by clip[1], in place; with a factor of 1 nothing is written.  rfx_grad_clip is one after
- * the other (a small set in one launch).  Gradients of one call that share memory are scaled one after the other.          */
-typedef struct rfx_grad_tensor {
-    void*   grad;                       /* dev [n] */
-    int64_t n;
-    int32_t dtype;
-    int32_t reserved;
-} rfx_grad_tensor;
-size_t rfx_grad_norm_workspace_bytes(const rfx_grad_tensor* tensors, int count);
+ * rfx_grad_scale multiplies the gradients by clip[1], in place; with a factor of 1 nothing is written.  rfx_grad_clip does both
+ * with a launch less.  Gradients of one call that share memory are scaled one after the other.                              */
+size_t rfx_grad_norm_workspace_bytes(int count);
 int rfx_grad_norm(const rfx_grad_tensor* tensors, int count, int norm_type, double max_norm, double* clip, float* norm32,
                   void* workspace, size_t workspace_bytes, rfx_stream stream);
-int rfx_grad_clip(const rfx_grad_tensor* tensors, int count, int norm_type, double max_norm, double* clip, float* norm32,
-                  void* workspace, size_t workspace_bytes, rfx_stream stream);
 int rfx_grad_scale(const rfx_grad_tensor* tensors, int count, const double* clip, rfx_stream stream);
+int rfx_grad_clip(const rfx_grad_tensor* tensors, int count, int norm_type, double max_norm, float* norm32, void* workspace,
+                  size_t workspace_bytes, rfx_stream stream);
 
 #ifdef __cplusplus
 }

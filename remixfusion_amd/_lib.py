@@ -212,11 +212,11 @@ PROTOTYPES = {
     "rfx_adamw_tensor_bytes": (C.c_size_t, []),
     "rfx_adamw_group_bytes": (C.c_size_t, []),
     "rfx_adamw_workspace_bytes": (C.c_size_t, [_i]),
-    "rfx_adamw_step": (_i, [_P, _i, _P, _i, _P, _P, _sz, _P]),
+    "rfx_adamw_step": (_i, [_P, _i, _P, _i, _P, C.c_double, _P, _P, _sz, _P]),
     "rfx_adamw_moments": (_i, [_P, _i, _P]),
-    "rfx_grad_norm_workspace_bytes": (C.c_size_t, [_P, _i]),
+    "rfx_grad_norm_workspace_bytes": (C.c_size_t, [_i]),
     "rfx_grad_norm": (_i, [_P, _i, _i, C.c_double, _P, _P, _P, _sz, _P]),
-    "rfx_grad_clip": (_i, [_P, _i, _i, C.c_double, _P, _P, _P, _sz, _P]),
+    "rfx_grad_clip": (_i, [_P, _i, _i, C.c_double, _P, _P, _sz, _P]),
     "rfx_grad_scale": (_i, [_P, _i, _P, _P]),
     "rfx_ba_workspace_bytes": (C.c_size_t, [_l, _i, _i, _i, _i]),
     "rfx_ba_forward_backward": (_i, [C.POINTER(BaDesc), _P, C.c_size_t, _P]),
@@ -289,7 +289,7 @@ def host():
         except ImportError as e:
             raise RfxError(f"_optim_host.so cannot be loaded ({e}): build it with `python -m remixfusion_amd.build`") from e
         _optim_host.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in (
-            "rfx_adamw_step", "rfx_adamw_workspace_bytes", "rfx_adamw_moments", "rfx_grad_norm_workspace_bytes", "rfx_grad_norm", "rfx_grad_clip")})
+            "rfx_adamw_step", "rfx_adamw_workspace_bytes", "rfx_adamw_moments", "rfx_grad_norm_workspace_bytes", "rfx_grad_clip")})
         _host = _optim_host
     return _host
 

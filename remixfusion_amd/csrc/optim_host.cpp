@@ -17,7 +17,6 @@ struct {
     decltype(&rfx_adamw_workspace_bytes) adamw_workspace_bytes;
     decltype(&rfx_adamw_moments) adamw_moments;
     decltype(&rfx_grad_norm_workspace_bytes) grad_norm_workspace_bytes;
-    decltype(&rfx_grad_norm) grad_norm;
     decltype(&rfx_grad_clip) grad_clip;
 } rfx;
 
@@ -27,7 +26,6 @@ void bind(const py::dict& at) {
     get("rfx_adamw_workspace_bytes", rfx.adamw_workspace_bytes);
     get("rfx_adamw_moments", rfx.adamw_moments);
     get("rfx_grad_norm_workspace_bytes", rfx.grad_norm_workspace_bytes);
-    get("rfx_grad_norm", rfx.grad_norm);
     get("rfx_grad_clip", rfx.grad_clip);
 }
 
@@ -96,7 +94,6 @@ class Plan {
     struct Settings { long state_bits; bool master, capturable; };
     std::vector<Settings> settings_;    // per parameter group
     at::Device device_;
-    size_t norm_bytes_ = 0;
     bool ordered_ = true, counted_ = false, host_counted_ = false;
 
     static Settings settings_of(PyObject* g) {
@@ -247,27 +244,18 @@ private:
             rows[i].group = (int32_t)at;
         }
         py::object norm = py::none();
-        at::Tensor ws, buf;
-        const double* clip = nullptr;
+        at::Tensor ws;
+        float* norm32 = nullptr;
+        const size_t bytes = limit >= 0.0 || counted_ ? rfx.adamw_workspace_bytes((int)n) : 0;
         if (limit >= 0.0) {
             for (size_t i = 0; i < n; ++i) grads_[i].grad = const_cast<void*>(rows[i].grad);
-            if (norm_bytes_ == 0) norm_bytes_ = rfx.grad_norm_workspace_bytes(grads_.data(), (int)n);
-            buf = at::empty({2 + (int64_t)norm_bytes_ / 8}, at::TensorOptions().dtype(at::kDouble).device(device_));
             at::Tensor out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device_));
-            double* at_clip = static_cast<double*>(buf.data_ptr());
-            const int rc = rfx.grad_norm(grads_.data(), (int)n, 2, limit, at_clip, static_cast<float*>(out.data_ptr()), at_clip + 2, norm_bytes_,
-                                         (rfx_stream)stream);
-            if (rc != RFX_OK) return py::int_(rc);
-            clip = at_clip;
+            norm32 = static_cast<float*>(out.data_ptr());
             norm = py::reinterpret_steal<py::object>(THPVariable_Wrap(out));
         }
-        size_t bytes = 0;
-        if (counted_) {
-            bytes = rfx.adamw_workspace_bytes((int)n);
-            ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(device_));
-        }
-        const int rc = rfx.adamw_step(rows.data(), (int)n, groups_.data(), (int)groups_.size(), clip, bytes ? ws.data_ptr() : nullptr, bytes,
-                                      (rfx_stream)stream);
+        if (bytes) ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(device_));
+        const int rc = rfx.adamw_step(rows.data(), (int)n, groups_.data(), (int)groups_.size(), limit >= 0.0 ? grads_.data() : nullptr, limit, norm32,
+                                      bytes ? ws.data_ptr() : nullptr, bytes, (rfx_stream)stream);
         if (rc != RFX_OK) return py::int_(rc);
         for (size_t i = 0; i < n; ++i)
             if (counts_[i]) *counts_[i] += 1.f;
@@ -293,11 +281,10 @@ py::object clip(const py::list& parameters, int kind, double limit, int device, 
         rows.push_back(r);
     }
     if (rows.empty()) return py::int_((int)OTHER_ORDER);
-    const size_t bytes = rfx.grad_norm_workspace_bytes(rows.data(), (int)rows.size());
-    at::Tensor buf = at::empty({2 + (int64_t)bytes / 8}, at::TensorOptions().dtype(at::kDouble).device(dev));
+    const size_t bytes = rfx.grad_norm_workspace_bytes((int)rows.size());
+    at::Tensor ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
     at::Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
-    double* at_clip = static_cast<double*>(buf.data_ptr());
-    const int rc = rfx.grad_clip(rows.data(), (int)rows.size(), kind, limit, at_clip, static_cast<float*>(norm.data_ptr()), at_clip + 2, bytes,
+    const int rc = rfx.grad_clip(rows.data(), (int)rows.size(), kind, limit, static_cast<float*>(norm.data_ptr()), ws.data_ptr(), bytes,
                                  (rfx_stream)stream);
     if (rc != RFX_OK) return py::int_(rc);
     return py::reinterpret_steal<py::object>(THPVariable_Wrap(norm));

@@ -43,12 +43,24 @@ struct AwGroup {
     float sign;                         // -1: maximize
 };
 
+// Where the clipping factor comes from: partial sums (maxima) of the norm that every block joins for itself -- at most as many as a
+// block has threads, so this is one load a thread out of L2 and a launch less -- or a factor that is there.  Neither: no clipping.
+constexpr int JOIN = 256;
+struct ClipSource {
+    const double* partial;
+    const double* factor;
+    double max_norm;
+    float* norm32;                      // written by the first block
+    int32_t n;
+    int32_t max;                        // maxima instead of sums of squares
+};
+
 struct AwArgs {
     AwTensor t[AW_TENSORS];
     int32_t first[AW_TENSORS + 1];
     AwGroup group[AW_GROUPS];
     const AwStep* dev;                  // per tensor of this launch, or null
-    const double* clip;
+    ClipSource clip;
     int32_t count;
 };
 static_assert(sizeof(AwArgs) <= 4096, "kernel arguments");
@@ -64,10 +76,17 @@ __device__ __forceinline__ f4 widen(vec4<float> x) { return x; }
 __device__ __forceinline__ f4 widen(vec4<__bf16> x) { return __builtin_convertvector(x, f4); }
 __device__ __forceinline__ f4 widen(vec4<_Float16> x) { return __builtin_convertvector(x, f4); }
 
-template <typename T> __device__ __forceinline__ f4 load4(const T* p) { return widen(*reinterpret_cast<const vec4<T>*>(p)); }
-template <typename T> __device__ __forceinline__ void store4(T* p, f4 x) {
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<f4*>(p) = x;
-    else *reinterpret_cast<vec4<T>*>(p) = __builtin_convertvector(x, vec4<T>);      // to nearest, ties to even: once, at the end
+// STREAM: past the caches, for sets that no cache holds until they are read again
+template <bool STREAM = false, typename T> __device__ __forceinline__ f4 load4(const T* p) {
+    const vec4<T>* at = reinterpret_cast<const vec4<T>*>(p);
+    return widen(STREAM ? __builtin_nontemporal_load(at) : *at);
+}
+template <bool STREAM = false, typename T> __device__ __forceinline__ void store4(T* p, f4 x) {
+    vec4<T> y;
+    if constexpr (sizeof(T) == 4) y = x;
+    else y = __builtin_convertvector(x, vec4<T>);                          // to nearest, ties to even: once, at the end
+    vec4<T>* at = reinterpret_cast<vec4<T>*>(p);
+    if (STREAM) __builtin_nontemporal_store(y, at); else *at = y;
 }
 
 // xor-shift / multiply mixer of 32-bit integers (a bijection)
@@ -112,14 +131,46 @@ __device__ __forceinline__ void adamw_one(float& p, float g, float& m, float& v,
     p = stepped(p, m, v, s, a.eps);
 }
 
-template <int TYPE, bool MASTER>
+__device__ __forceinline__ double larger(double p, double q) { return p != p ? p : (q != q || q > p) ? q : p; }     // NaN wins
+
+template <int THREADS> __device__ __forceinline__ double block_join(double x, bool max, double* lds) {      // every thread gets it; fixed order
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        const double y = __shfl_xor(x, d, 64);
+        x = max ? larger(x, y) : x + y;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = lds[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) x = max ? larger(x, lds[w]) : x + lds[w];
+    return x;
+}
+
+__device__ __forceinline__ double factor_of(double norm, double max_norm) {
+    const double f = max_norm / (norm + 1e-6);
+    return f > 1.0 ? 1.0 : f;                                              // NaN stays NaN
+}
+
+// for blocks of JOIN threads
+__device__ __forceinline__ double clip_factor(const ClipSource& c) {
+    if (c.n == 0) return c.factor ? c.factor[1] : 1.0;
+    __shared__ double lds[JOIN / 64];
+    const double x = block_join<JOIN>((int)threadIdx.x < c.n ? c.partial[threadIdx.x] : 0.0, c.max != 0, lds);
+    const double norm = c.max ? x : sqrt(x);
+    if (c.norm32 && blockIdx.x == 0 && threadIdx.x == 0) *c.norm32 = (float)norm;
+    return factor_of(norm, c.max_norm);
+}
+
+template <int TYPE, bool MASTER, bool STREAM>
 __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(const AwArgs k) {
     typedef typename Elem<TYPE>::T T;
     const int ti = find(k.first, k.count, (int)blockIdx.x);
     const AwTensor& t = k.t[ti];
     const AwGroup& a = k.group[t.group];
     const AwStep s = k.dev ? k.dev[ti] : a.s;
-    const float c = a.sign * (k.clip ? (float)k.clip[1] : 1.f);
+    const float c = a.sign * (float)clip_factor(k.clip);
     const int64_t base = (int64_t)((int)blockIdx.x - k.first[ti]) * AW_PIECE;
     const int len = (int)(t.n - base < AW_PIECE ? t.n - base : AW_PIECE);
     T* p = (T*)t.p + base;
@@ -132,19 +183,19 @@ __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(const AwArgs k) {
     if (vec) {
         done = len & ~3;
         for (int i = threadIdx.x * 4; i < done; i += AW_THREADS * 4) {
-            f4 x = MASTER ? load4(w + i) : load4(p + i);
-            const f4 gg = load4(g + i);
-            f4 mm = load4(m + i), vv = load4(v + i);
+            f4 x = MASTER ? load4<STREAM>(w + i) : load4<STREAM>(p + i);
+            const f4 gg = load4<STREAM>(g + i);
+            f4 mm = load4<STREAM>(m + i), vv = load4<STREAM>(v + i);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float xj = x[j], mj = mm[j], vj = vv[j];
                 adamw_one(xj, gg[j], mj, vj, a, s, c);
                 x[j] = xj; mm[j] = mj; vv[j] = vj;
             }
-            store4(p + i, x);
-            if (MASTER) store4(w + i, x);
-            store4(m + i, mm);
-            store4(v + i, vv);
+            store4<STREAM>(p + i, x);
+            if (MASTER) store4<STREAM>(w + i, x);
+            store4<STREAM>(m + i, mm);
+            store4<STREAM>(v + i, vv);
         }
     }
     for (int i = done + threadIdx.x; i < len; i += AW_THREADS) {
@@ -160,18 +211,23 @@ __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(const AwArgs k) {
 // A wave owns a run of 256 elements, four consecutive ones a lane.  The moments are formed in fp64 (full rate on this chip), so
 // that which side of a border they fall on does not depend on the order of the operations; the update is fp32.
 //   decode: a byte's seven (eight) bits moved to an fp32's exponent and mantissa ARE the format, subnormals included, times a power
-//           of two that is a constant of the run;
+//           of two that is a constant of the run (beta goes into it: a product with a power of two is exact);
 //   encode: the moment times the inverse power of two, rounded to fp32 (subnormals included), leaves 20 bits below the format's
 //           last place: 16 random bits (and half of their unit) are added, and the upper bits are the code.
 __device__ __forceinline__ double pow2(int e) { return __longlong_as_double((long long)(e + 1023) << 52); }
 
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const uint32_t y = (uint32_t)__shfl_xor((int)x, d, 64);
-        x = x > y ? x : y;
-    }
-    return x;
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+    const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);       // lanes without a source: 0
+    return x > y ? x : y;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {                 // a scalar
+    x = dpp_max<0x111, 0xf>(x);                                            // from the lane 1, 2, 4, 8 to the left in a row of 16
+    x = dpp_max<0x112, 0xf>(x);
+    x = dpp_max<0x114, 0xf>(x);
+    x = dpp_max<0x118, 0xf>(x);
+    x = dpp_max<0x142, 0xa>(x);                                            // a row's last lane to the next row
+    x = dpp_max<0x143, 0xc>(x);                                            // lane 31 to the upper half
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
 // exponent byte of a run from the upper word of its largest magnitude (an fp64's bits order like integers, NaN above all).
@@ -186,91 +242,133 @@ template <int UNIT> __device__ __forceinline__ int run_exponent(uint32_t hi) {
 __device__ __forceinline__ double scale_m(int byte) { return byte == -128 ? __builtin_nan("") : pow2(byte + 112); }
 __device__ __forceinline__ double scale_v(int byte) { return byte == -128 ? __builtin_nan("") : pow2(2 * byte + 96); }
 
-template <int TOP> __device__ __forceinline__ uint32_t encode(double mag, double inverse, uint32_t r16) {
-    const uint32_t z = __float_as_uint((float)(mag * inverse)) + (r16 << 4) + 8;
-    const uint32_t c = z >> 20;
-    return c < (uint32_t)TOP ? c : (uint32_t)TOP;
+template <int J> __device__ __forceinline__ float bits_m(uint32_t codes) {
+    const uint32_t x = codes << (24 - 8 * J);
+    return __uint_as_float((x & 0x80000000U) | ((x >> 4) & 0x07f00000U));
+}
+template <int J> __device__ __forceinline__ float bits_v(uint32_t codes) {
+    return __uint_as_float((J < 3 ? codes << (24 - 8 * J) : codes) >> 4 & 0x0ff00000U);
 }
 
-template <int TYPE, bool MASTER>
+template <uint32_t TOP> __device__ __forceinline__ uint32_t encode(double magnitude, double inverse, uint32_t noise) {
+    const uint32_t c = (__float_as_uint((float)(magnitude * inverse)) + noise) >> 20;
+    return c < TOP ? c : TOP;
+}
+
+struct Run8 {                           // a lane's share of a run as it is loaded
+    f4 x, g;
+    uint32_t cm, cv;
+    int e1, e2;
+};
+
+// new moments of a lane's elements (codes in r.cm, r.cv), the stepped parameter in r.x, the run's exponents in r.e1, r.e2
+template <bool FULL> __device__ __forceinline__ void adamw8_run(Run8& r, const AwGroup& a, const AwStep& s, double c, uint32_t run_key, int lane, int have) {
+    const double s1 = scale_m(__builtin_amdgcn_readfirstlane(r.e1)) * a.b1, s2 = scale_v(__builtin_amdgcn_readfirstlane(r.e2)) * a.b2;
+    const float bm[4] = {bits_m<0>(r.cm), bits_m<1>(r.cm), bits_m<2>(r.cm), bits_m<3>(r.cm)};
+    const float bv[4] = {bits_v<0>(r.cv), bits_v<1>(r.cv), bits_v<2>(r.cv), bits_v<3>(r.cv)};
+    double m[4], v[4];
+    uint32_t h1 = 0, h2 = 0, u2[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const double g = (double)r.g[j] * c;
+        m[j] = fma(g, a.c1, (double)bm[j] * s1);
+        v[j] = fma(g * g, a.c2, (double)bv[j] * s2);
+        const uint32_t u1 = (uint32_t)__double2hiint(m[j]) & 0x7fffffffU;
+        u2[j] = (uint32_t)__double2hiint(v[j]) & 0x7fffffffU;
+        if (FULL || j < have) { h1 = h1 > u1 ? h1 : u1; h2 = h2 > u2[j] ? h2 : u2[j]; }
+    }
+    r.e1 = run_exponent<1>(wave_max(h1));
+    r.e2 = run_exponent<2>(wave_max(h2));
+    const double i1 = pow2(-112 - r.e1), i2 = pow2(-96 - 2 * r.e2);
+    r.cm = r.cv = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t bits = mix32(run_key + (uint32_t)(lane * 4 + j) * 0x9e3779b9U);
+        // 16 bits at the place 2^4 of the 20, and half of a unit of theirs
+        const uint32_t cm = encode<127>(fabs(m[j]), i1, ((bits & 0xffffU) << 4) | 8U);
+        uint32_t cv = encode<255>(v[j], i2, (bits >> 16 << 4) | 8U);
+        const uint32_t some = u2[j] < 1U ? u2[j] : 1U;                     // v > 0 stays above 0: m / eps would be a leap
+        cv = cv > some ? cv : some;
+        r.cm |= (cm | ((uint32_t)__double2hiint(m[j]) >> 24 & 128U)) << (8 * j);
+        r.cv |= cv << (8 * j);
+        // fp32, the chip's own root and reciprocal (an ulp each, under 16 u of the update all told).  They take subnormals for 0: a
+        // second moment under 2^-126 counts as that much
+        const float root = __builtin_amdgcn_sqrtf(fmaxf((float)v[j], 1.17549435e-38f));
+        const float d = madd(root, s.inv_bc2, a.eps);
+        r.x[j] -= madd(s.lr_wd, r.x[j], s.step_size * ((float)m[j] * __builtin_amdgcn_rcpf(d)));
+    }
+}
+
+template <int TYPE, bool MASTER, bool STREAM>
 __global__ __launch_bounds__(AW_THREADS) void adamw8_kernel(const AwArgs k) {
     typedef typename Elem<TYPE>::T T;
     const int ti = find(k.first, k.count, (int)blockIdx.x);
     const AwTensor& t = k.t[ti];
     const AwGroup& a = k.group[t.group];
     const AwStep s = k.dev ? k.dev[ti] : a.s;
-    const double c = (double)a.sign * (k.clip ? k.clip[1] : 1.0);
+    const double c = (double)a.sign * clip_factor(k.clip);
     const int64_t piece = (int)blockIdx.x - k.first[ti];
     const int64_t base = piece * AW_PIECE;
     const int len = (int)(t.n - base < AW_PIECE ? t.n - base : AW_PIECE);
-    const int64_t runs = (t.n + AW_RUN - 1) / AW_RUN;
-    const uint32_t key = mix32(s.key + t.index);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t runs = (t.n + AW_RUN - 1) / AW_RUN, run0 = piece * (AW_PIECE / AW_RUN);
+    const uint32_t key = mix32(s.key + t.index) + (uint32_t)run0;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const T* g = (const T*)t.g + base;
     T* p = (T*)t.p + base;
     float* w = MASTER ? t.w + base : nullptr;
     uint8_t* m = (uint8_t*)t.m + base;
     uint8_t* v = (uint8_t*)t.v + base;
+    int8_t* e1 = t.e + run0;
+    int8_t* e2 = t.e + runs + run0;
     const bool vec = ((((uintptr_t)p | (uintptr_t)g) & (4 * sizeof(T) - 1)) | ((uintptr_t)w & 15)) == 0;
-    for (int r = wave; r * AW_RUN < len; r += AW_THREADS / 64) {
-        const int64_t run = piece * (AW_PIECE / AW_RUN) + r;
-        const int i = r * AW_RUN + lane * 4;
-        const int have = len - i < 0 ? 0 : len - i > 4 ? 4 : len - i;  // elements of this lane
-        f4 x = {0, 0, 0, 0}, gg = {0, 0, 0, 0};
-        uint32_t cm = 0, cv = 0;
-        if (have == 4 && vec) {
-            x = MASTER ? load4(w + i) : load4(p + i);
-            gg = load4(g + i);
-        } else {
-            for (int j = 0; j < have; ++j) { x[j] = MASTER ? w[i + j] : (float)p[i + j]; gg[j] = (float)g[i + j]; }
-        }
-        if (have == 4) {
-            cm = *reinterpret_cast<const uint32_t*>(m + i);
-            cv = *reinterpret_cast<const uint32_t*>(v + i);
-        } else {
-            for (int j = 0; j < have; ++j) { cm |= (uint32_t)m[i + j] << (8 * j); cv |= (uint32_t)v[i + j] << (8 * j); }
-        }
-        const double s1 = scale_m(t.e[run]), s2 = scale_v(t.e[runs + run]);
-        double md[4], vd[4];
-        uint32_t h1 = 0, h2 = 0;
+    if (len == AW_PIECE && vec) {
+        constexpr int MINE = AW_PIECE / AW_RUN / (AW_THREADS / 64);        // runs of a wave, the next one's loads on their way while one is stepped
+        const auto load = [&](int r) {
+            const int i = (wave + r * (AW_THREADS / 64)) * AW_RUN + lane * 4;
+            Run8 x;
+            x.x = MASTER ? load4<STREAM>(w + i) : load4<STREAM>(p + i);
+            x.g = load4<STREAM>(g + i);
+            x.cm = *reinterpret_cast<const uint32_t*>(m + i);
+            x.cv = *reinterpret_cast<const uint32_t*>(v + i);
+            x.e1 = e1[wave + r * (AW_THREADS / 64)];
+            x.e2 = e2[wave + r * (AW_THREADS / 64)];
+            return x;
+        };
+        Run8 next = load(0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t bm = (cm >> (8 * j)) & 255, bv = (cv >> (8 * j)) & 255;
-            const double gd = (double)gg[j] * c;
-            md[j] = (double)__uint_as_float((bm & 127) << 20 | (bm & 128) << 24) * s1 * a.b1 + gd * a.c1;
-            vd[j] = (double)__uint_as_float(bv << 20) * s2 * a.b2 + gd * gd * a.c2;
-            const uint32_t u1 = (uint32_t)__double2hiint(md[j]) & 0x7fffffffU, u2 = (uint32_t)__double2hiint(vd[j]) & 0x7fffffffU;
-            if (j < have) { h1 = h1 > u1 ? h1 : u1; h2 = h2 > u2 ? h2 : u2; }
+        for (int r = 0; r < MINE; ++r) {
+            Run8 x = next;
+            if (r + 1 < MINE) next = load(r + 1);
+            const int run = wave + r * (AW_THREADS / 64), i = run * AW_RUN + lane * 4;
+            adamw8_run<true>(x, a, s, c, mix32(key + (uint32_t)run), lane, 4);
+            store4<STREAM>(p + i, x.x);
+            if (MASTER) store4<STREAM>(w + i, x.x);
+            *reinterpret_cast<uint32_t*>(m + i) = x.cm;
+            *reinterpret_cast<uint32_t*>(v + i) = x.cv;
+            if (lane == 0) { e1[run] = (int8_t)x.e1; e2[run] = (int8_t)x.e2; }
         }
-        const int n1 = run_exponent<1>(wave_max(h1)), n2 = run_exponent<2>(wave_max(h2));
-        const double i1 = pow2(-112 - n1), i2 = pow2(-96 - 2 * n2);
-        const uint32_t hash = mix32(key + (uint32_t)run);
-        cm = 0; cv = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t r16 = mix32(hash + (uint32_t)(lane * 4 + j) * 0x9e3779b9U);
-            uint32_t bm = encode<127>(fabs(md[j]), i1, r16 & 0xffff), bv = encode<255>(vd[j], i2, r16 >> 16);
-            if (vd[j] > 0.0 && bv == 0) bv = 1;
-            if (n1 == -128) bm = 0;
-            if (n2 == -128) bv = 0;
-            bm |= md[j] < 0.0 ? 128 : 0;
-            cm |= bm << (8 * j);
-            cv |= bv << (8 * j);
-            x[j] = stepped(x[j], (float)md[j], (float)vd[j], s, a.eps);
+        return;
+    }
+    for (int run = wave; run * AW_RUN < len; run += AW_THREADS / 64) {     // a tensor's last piece, or one that vector loads do not fit
+        const int i = run * AW_RUN + lane * 4;
+        const int have = len - i < 0 ? 0 : len - i > 4 ? 4 : len - i;      // elements of this lane
+        Run8 x{};
+        for (int j = 0; j < have; ++j) {
+            x.x[j] = MASTER ? w[i + j] : (float)p[i + j];
+            x.g[j] = (float)g[i + j];
+            x.cm |= (uint32_t)m[i + j] << (8 * j);
+            x.cv |= (uint32_t)v[i + j] << (8 * j);
         }
-        if (have == 4 && vec) {
-            store4(p + i, x);
-            if (MASTER) store4(w + i, x);
-        } else {
-            for (int j = 0; j < have; ++j) { p[i + j] = (T)x[j]; if (MASTER) w[i + j] = x[j]; }
+        x.e1 = e1[run];
+        x.e2 = e2[run];
+        adamw8_run<false>(x, a, s, c, mix32(key + (uint32_t)run), lane, have);
+        for (int j = 0; j < have; ++j) {
+            p[i + j] = (T)x.x[j];
+            if (MASTER) w[i + j] = x.x[j];
+            m[i + j] = (uint8_t)(x.cm >> (8 * j));
+            v[i + j] = (uint8_t)(x.cv >> (8 * j));
         }
-        if (have == 4) {
-            *reinterpret_cast<uint32_t*>(m + i) = cm;
-            *reinterpret_cast<uint32_t*>(v + i) = cv;
-        } else {
-            for (int j = 0; j < have; ++j) { m[i + j] = (uint8_t)(cm >> (8 * j)); v[i + j] = (uint8_t)(cv >> (8 * j)); }
-        }
-        if (lane == 0) { t.e[run] = (int8_t)n1; t.e[runs + run] = (int8_t)n2; }
+        if (lane == 0) { e1[run] = (int8_t)x.e1; e2[run] = (int8_t)x.e2; }
     }
 }
 
@@ -301,6 +399,7 @@ struct MomArgs {
 };
 static_assert(sizeof(MomArgs) <= 4096, "kernel arguments");
 
+template <bool STREAM>
 __global__ __launch_bounds__(AW_THREADS) void adamw_moments_kernel(const MomArgs k) {
     const int ti = find(k.first, k.count, (int)blockIdx.x);
     const rfx_moment_tensor& t = k.t[ti];
@@ -323,76 +422,57 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_moments_kernel(const MomArgs
         } else {
             for (int j = 0; j < have; ++j) { cm |= (uint32_t)m[i + j] << (8 * j); cv |= (uint32_t)v[i + j] << (8 * j); }
         }
-        f4 a, b;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t bm = (cm >> (8 * j)) & 255, bv = (cv >> (8 * j)) & 255;
-            a[j] = (float)((double)__uint_as_float((bm & 127) << 20 | (bm & 128) << 24) * s1);
-            b[j] = (float)((double)__uint_as_float(bv << 20) * s2);
-        }
+        const auto value = [](float bits, double scale) { return (float)((double)bits * scale); };
+        const f4 a = {value(bits_m<0>(cm), s1), value(bits_m<1>(cm), s1), value(bits_m<2>(cm), s1), value(bits_m<3>(cm), s1)};
+        const f4 b = {value(bits_v<0>(cv), s2), value(bits_v<1>(cv), s2), value(bits_v<2>(cv), s2), value(bits_v<3>(cv), s2)};
         if (have == 4 && vec) {
-            store4(om + i, a);
-            store4(ov + i, b);
+            store4<STREAM>(om + i, a);
+            store4<STREAM>(ov + i, b);
         } else {
             for (int j = 0; j < have; ++j) { om[i + j] = a[j]; ov[i + j] = b[j]; }
         }
     }
 }
 
-// ---- global norm ------------------------------------------------------------------------------------------------------------
+// ---- global norm --------------------------------------------------------------------------------------------------------------
+// One block per CU at most (16 waves, four loads of each in flight: enough to draw what HBM gives), so that there are never more
+// partial results than the blocks that read them join with one load a thread.  Pieces are dealt in turn: at least eight a block
+// where there is much, so that the last round weighs little.
 constexpr int GN_TENSORS = 128;
-constexpr int GN_THREADS = 256;
-constexpr int GN_PIECE = 16384;
-constexpr int GN_BLOCKS = 1024;         // partial sums of a launch at most
+constexpr int GN_THREADS = 1024;
+constexpr int GN_LEAST = 4096;          // elements of a piece: one float4 a thread
+constexpr int GN_MOST = 65536;
 
 struct GnArgs {
     struct { void* g; int64_t n; } t[GN_TENSORS];
     int32_t first[GN_TENSORS + 1];
     uint8_t dtype[GN_TENSORS];
     double* partial;
-    const double* clip;
-    int32_t count, pieces, kind;
+    ClipSource clip;
+    int32_t count, pieces, piece, max;
 };
 static_assert(sizeof(GnArgs) <= 4096, "kernel arguments");
 
 template <typename T, bool MAX> __device__ __forceinline__ void norm_piece(const T* g, int len, double& sum, uint32_t& big) {
     int done = 0;
-    auto one = [&](float x) {
+    const auto one = [&](float x) {
         if (MAX) { const uint32_t u = __float_as_uint(x) & 0x7fffffffU; big = big > u ? big : u; }      // integers order NaN above all
         else { const double d = (double)x; sum = fma(d, d, sum); }
     };
+    const auto four = [&](f4 x) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) one(x[j]);
+    };
     if (((uintptr_t)g & (4 * sizeof(T) - 1)) == 0) {
         done = len & ~3;
-        for (int i = threadIdx.x * 4; i < done; i += GN_THREADS * 4) {
-            const f4 x = load4(g + i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) one(x[j]);
+        int i = threadIdx.x * 4;
+        for (; i + 3 * GN_THREADS * 4 < done; i += 4 * GN_THREADS * 4) {
+            const f4 a = load4(g + i), b = load4(g + i + GN_THREADS * 4), c = load4(g + i + 2 * GN_THREADS * 4), d = load4(g + i + 3 * GN_THREADS * 4);
+            four(a); four(b); four(c); four(d);
         }
+        for (; i < done; i += GN_THREADS * 4) four(load4(g + i));
     }
     for (int i = done + threadIdx.x; i < len; i += GN_THREADS) one((float)g[i]);
-}
-
-__device__ __forceinline__ double block_sum(double x, double* lds) {       // every thread gets the sum; fixed order
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-    __syncthreads();
-    double s = 0.0;
-    for (int w = 0; w < GN_THREADS / 64; ++w) s += lds[w];
-    return s;
-}
-
-__device__ __forceinline__ double block_max(double x, double* lds) {       // of non-negative values; NaN wins
-    const auto larger = [](double p, double q) { return p != p ? p : (q != q || q > p) ? q : p; };
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) x = larger(x, __shfl_xor(x, d, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-    __syncthreads();
-    double s = 0.0;
-    for (int w = 0; w < GN_THREADS / 64; ++w) s = larger(s, lds[w]);
-    return s;
 }
 
 template <bool MAX>
@@ -402,50 +482,52 @@ __global__ __launch_bounds__(GN_THREADS) void grad_norm_kernel(const GnArgs k) {
     uint32_t big = 0;
     for (int piece = blockIdx.x; piece < k.pieces; piece += gridDim.x) {
         const int ti = find(k.first, k.count, piece);
-        const int64_t base = (int64_t)(piece - k.first[ti]) * GN_PIECE, n = k.t[ti].n;
-        const int len = (int)(n - base < GN_PIECE ? n - base : GN_PIECE);
+        const int64_t base = (int64_t)(piece - k.first[ti]) * k.piece, n = k.t[ti].n;
+        const int len = (int)(n - base < k.piece ? n - base : k.piece);
         if (k.dtype[ti] == RFX_F32) norm_piece<float, MAX>((const float*)k.t[ti].g + base, len, sum, big);
         else if (k.dtype[ti] == RFX_BF16) norm_piece<__bf16, MAX>((const __bf16*)k.t[ti].g + base, len, sum, big);
         else norm_piece<_Float16, MAX>((const _Float16*)k.t[ti].g + base, len, sum, big);
     }
-    const double r = MAX ? block_max((double)__uint_as_float(big), lds) : block_sum(sum, lds);
+    const double r = block_join<GN_THREADS>(MAX ? (double)__uint_as_float(big) : sum, MAX, lds);
     if (threadIdx.x == 0) k.partial[blockIdx.x] = r;
 }
 
-template <bool MAX>
-__global__ __launch_bounds__(GN_THREADS) void grad_norm_join_kernel(const double* partial, int n, double max_norm, double* clip, float* norm32) {
-    __shared__ double lds[GN_THREADS / 64];
+// many partial results (of several launches) to one, or to the norm and its factor
+__global__ __launch_bounds__(JOIN) void grad_norm_join_kernel(const double* partial, int n, int max, double max_norm, double* one, double* clip,
+                                                              float* norm32) {
+    __shared__ double lds[JOIN / 64];
     double x = 0.0;
-    for (int i = threadIdx.x; i < n; i += GN_THREADS) {
-        if (MAX) x = x != x ? x : (partial[i] != partial[i] || partial[i] > x) ? partial[i] : x;
-        else x += partial[i];
+    for (int i = threadIdx.x; i < n; i += JOIN) x = max ? larger(x, partial[i]) : x + partial[i];
+    x = block_join<JOIN>(x, max != 0, lds);
+    if (threadIdx.x != 0) return;
+    if (one) { *one = x; return; }
+    const double norm = max ? x : sqrt(x);
+    if (clip) {
+        clip[0] = norm;
+        clip[1] = factor_of(norm, max_norm);
     }
-    x = MAX ? block_max(x, lds) : sqrt(block_sum(x, lds));
-    if (threadIdx.x == 0) {
-        const double f = max_norm / (x + 1e-6);
-        clip[0] = x;
-        clip[1] = f > 1.0 ? 1.0 : f;                                       // NaN stays NaN
-        if (norm32) *norm32 = (float)x;
-    }
+    if (norm32) *norm32 = (float)norm;
 }
 
+constexpr int SC_THREADS = JOIN;
+constexpr int SC_BLOCKS = 2048;         // eight a CU: what is resident at once
 template <typename T> __device__ __forceinline__ void scale_piece(T* g, int len, float c) {
     int done = 0;
     if (((uintptr_t)g & (4 * sizeof(T) - 1)) == 0) {
         done = len & ~3;
-        for (int i = threadIdx.x * 4; i < done; i += GN_THREADS * 4) store4(g + i, load4(g + i) * c);
+        for (int i = threadIdx.x * 4; i < done; i += SC_THREADS * 4) store4(g + i, load4(g + i) * c);
     }
-    for (int i = done + threadIdx.x; i < len; i += GN_THREADS) g[i] = (T)((float)g[i] * c);
+    for (int i = done + threadIdx.x; i < len; i += SC_THREADS) g[i] = (T)((float)g[i] * c);
 }
 
-__global__ __launch_bounds__(GN_THREADS) void grad_scale_kernel(const GnArgs k) {
-    const double f = k.clip[1];
+__global__ __launch_bounds__(SC_THREADS) void grad_scale_kernel(const GnArgs k) {
+    const double f = clip_factor(k.clip);
     if (f == 1.0) return;
     const float c = (float)f;
     for (int piece = blockIdx.x; piece < k.pieces; piece += gridDim.x) {
         const int ti = find(k.first, k.count, piece);
-        const int64_t base = (int64_t)(piece - k.first[ti]) * GN_PIECE, n = k.t[ti].n;
-        const int len = (int)(n - base < GN_PIECE ? n - base : GN_PIECE);
+        const int64_t base = (int64_t)(piece - k.first[ti]) * k.piece, n = k.t[ti].n;
+        const int len = (int)(n - base < k.piece ? n - base : k.piece);
         if (k.dtype[ti] == RFX_F32) scale_piece((float*)k.t[ti].g + base, len, c);
         else if (k.dtype[ti] == RFX_BF16) scale_piece((__bf16*)k.t[ti].g + base, len, c);
         else scale_piece((_Float16*)k.t[ti].g + base, len, c);
@@ -455,8 +537,13 @@ __global__ __launch_bounds__(GN_THREADS) void grad_scale_kernel(const GnArgs k) 
 // ---- host -------------------------------------------------------------------------------------------------------------------
 static int elem_bytes(int dtype) { return dtype == RFX_F32 ? 4 : 2; }
 
+// From this much memory on (parameters, gradients, moments) the step's loads and stores go past the caches.
+// Measured, us a step (plain loads and stores / past the caches): 26 MB of fp32 tensors stepped again and again 9.5 / 11.6, 64 MB 19.6 / 25,
+// 128 MB 46 / 43, 665 MB 222 / 204; behind other work on 256 MB, as in a training loop, 16 MB 13.8 / 8.1, 64 MB 44 / 26, 128 MB 68 / 44.
+constexpr int64_t STREAM_BYTES = 64 << 20;
+
 // one launch of the tensors gathered in `k`; dev: their scalars' place in the workspace (step counts on the device)
-static int adamw_launch(AwArgs& k, PrepArgs* prep, int kind, hipStream_t stream) {
+static int adamw_launch(AwArgs& k, PrepArgs* prep, int kind, bool stream_past, hipStream_t stream) {
     if (k.count == 0) return RFX_OK;
     if (prep) {
         prep->count = k.count;
@@ -469,22 +556,26 @@ static int adamw_launch(AwArgs& k, PrepArgs* prep, int kind, hipStream_t stream)
         k.count = 0;
         return RFX_OK;
     }
-    const dim3 grid((unsigned)k.first[k.count]), block(AW_THREADS);
+    const void* kernel = nullptr;
+    const auto pick = [&](auto plain, auto streaming) { kernel = stream_past ? (const void*)streaming : (const void*)plain; };
     switch (kind) {
-        case 0: hipLaunchKernelGGL((adamw32_kernel<RFX_F32, false>), grid, block, 0, stream, k); break;
-        case 1: hipLaunchKernelGGL((adamw32_kernel<RFX_BF16, false>), grid, block, 0, stream, k); break;
-        case 2: hipLaunchKernelGGL((adamw32_kernel<RFX_F16, false>), grid, block, 0, stream, k); break;
-        case 4: hipLaunchKernelGGL((adamw32_kernel<RFX_BF16, true>), grid, block, 0, stream, k); break;
-        case 5: hipLaunchKernelGGL((adamw32_kernel<RFX_F16, true>), grid, block, 0, stream, k); break;
-        case 6: hipLaunchKernelGGL((adamw8_kernel<RFX_F32, false>), grid, block, 0, stream, k); break;
-        case 7: hipLaunchKernelGGL((adamw8_kernel<RFX_BF16, false>), grid, block, 0, stream, k); break;
-        case 8: hipLaunchKernelGGL((adamw8_kernel<RFX_F16, false>), grid, block, 0, stream, k); break;
-        case 10: hipLaunchKernelGGL((adamw8_kernel<RFX_BF16, true>), grid, block, 0, stream, k); break;
-        case 11: hipLaunchKernelGGL((adamw8_kernel<RFX_F16, true>), grid, block, 0, stream, k); break;
+        case 0: pick(adamw32_kernel<RFX_F32, false, false>, adamw32_kernel<RFX_F32, false, true>); break;
+        case 1: pick(adamw32_kernel<RFX_BF16, false, false>, adamw32_kernel<RFX_BF16, false, true>); break;
+        case 2: pick(adamw32_kernel<RFX_F16, false, false>, adamw32_kernel<RFX_F16, false, true>); break;
+        case 4: pick(adamw32_kernel<RFX_BF16, true, false>, adamw32_kernel<RFX_BF16, true, true>); break;
+        case 5: pick(adamw32_kernel<RFX_F16, true, false>, adamw32_kernel<RFX_F16, true, true>); break;
+        case 6: pick(adamw8_kernel<RFX_F32, false, false>, adamw8_kernel<RFX_F32, false, true>); break;
+        case 7: pick(adamw8_kernel<RFX_BF16, false, false>, adamw8_kernel<RFX_BF16, false, true>); break;
+        case 8: pick(adamw8_kernel<RFX_F16, false, false>, adamw8_kernel<RFX_F16, false, true>); break;
+        case 10: pick(adamw8_kernel<RFX_BF16, true, false>, adamw8_kernel<RFX_BF16, true, true>); break;
+        case 11: pick(adamw8_kernel<RFX_F16, true, false>, adamw8_kernel<RFX_F16, true, true>); break;
         default: return RFX_ERR_ARG;
     }
+    void* args[] = {&k};
+    RFX_HIP_TRY(hipLaunchKernel(kernel, dim3((unsigned)k.first[k.count]), dim3(AW_THREADS), args, 0, stream));
     RFX_LAUNCH_CHECK();
     k.count = 0;
+    k.clip.norm32 = nullptr;                                               // the first launch has written it
     return RFX_OK;
 }
 
@@ -514,9 +605,10 @@ static bool overlap(const rfx_adamw_tensor& a, const rfx_adamw_tensor& b) {
 
 // pieces of the gradients [at, at + as many as fit) as one launch; returns how many were taken, 0: none left, < 0: an error.
 // apart: no two of a launch share memory (they are written)
-static int gather(const rfx_grad_tensor* t, int count, int& at, GnArgs& k, bool apart) {
+static int gather(const rfx_grad_tensor* t, int count, int& at, GnArgs& k, int piece, bool apart) {
     int64_t pieces = 0;
     k.count = 0;
+    k.piece = piece;
     for (; at < count && k.count < GN_TENSORS; ++at) {
         if (t[at].n == 0) continue;
         bool shared = false;
@@ -525,7 +617,7 @@ static int gather(const rfx_grad_tensor* t, int count, int& at, GnArgs& k, bool 
             shared = a < b + (uintptr_t)k.t[j].n * elem_bytes(k.dtype[j]) && b < a + (uintptr_t)t[at].n * elem_bytes(t[at].dtype);
         }
         if (shared) break;
-        const int64_t p = (t[at].n + GN_PIECE - 1) / GN_PIECE;
+        const int64_t p = (t[at].n + piece - 1) / piece;
         if (p > 0x7fffffff) return RFX_ERR_UNSUPPORTED;
         if (pieces + p > 0x7fffffff) break;
         k.t[k.count].g = t[at].grad;
@@ -547,7 +639,68 @@ static bool grads_ok(const rfx_grad_tensor* t, int count) {
     return true;
 }
 
-static int norm_blocks(int pieces) { return pieces < GN_BLOCKS ? pieces : GN_BLOCKS; }
+// elements of a piece: eight pieces for each of the norm's blocks, in whole rounds of a block
+static int piece_of(const rfx_grad_tensor* t, int count) {
+    int64_t all = 0;
+    for (int i = 0; i < count; ++i) all += t[i].n;
+    int64_t piece = (all / (8 * JOIN) + GN_LEAST - 1) / GN_LEAST * GN_LEAST;
+    return (int)(piece < GN_LEAST ? GN_LEAST : piece > GN_MOST ? GN_MOST : piece);
+}
+
+static size_t partials(int count) { return (size_t)JOIN * ((count + GN_TENSORS - 1) / GN_TENSORS) + 1; }
+
+// partial results of the norm; `from`: how a kernel finds the factor in them
+static int norm_launches(const rfx_grad_tensor* tensors, int count, int max, double max_norm, double* workspace, int& n, ClipSource& from,
+                         hipStream_t stream) {
+    GnArgs k;
+    const int piece = piece_of(tensors, count);
+    n = 0;
+    for (int at = 0;;) {
+        const int taken = gather(tensors, count, at, k, piece, false);
+        if (taken < 0) return taken;
+        if (taken == 0) break;
+        const int blocks = k.pieces < JOIN ? k.pieces : JOIN;
+        k.partial = workspace + n;
+        n += blocks;
+        if (max) hipLaunchKernelGGL(grad_norm_kernel<true>, dim3(blocks), dim3(GN_THREADS), 0, stream, k);
+        else hipLaunchKernelGGL(grad_norm_kernel<false>, dim3(blocks), dim3(GN_THREADS), 0, stream, k);
+        RFX_LAUNCH_CHECK();
+    }
+    from = ClipSource{workspace, nullptr, max_norm, nullptr, n, max};
+    return RFX_OK;
+}
+
+// ... and at most as many of them as a kernel's block joins by itself
+static int few(double* workspace, int n, ClipSource& from, hipStream_t stream) {
+    if (n <= JOIN) return RFX_OK;                                          // (none: no element, and nothing that would ask)
+    hipLaunchKernelGGL(grad_norm_join_kernel, dim3(1), dim3(JOIN), 0, stream, workspace, n, from.max, 0.0, workspace + n, nullptr, nullptr);
+    RFX_LAUNCH_CHECK();
+    from.partial = workspace + n;
+    from.n = 1;
+    return RFX_OK;
+}
+
+// the norm of no element at all, which no other launch of the call has written
+static int no_norm(const double* workspace, float* norm32, hipStream_t stream) {
+    if (!norm32) return RFX_OK;
+    hipLaunchKernelGGL(grad_norm_join_kernel, dim3(1), dim3(JOIN), 0, stream, workspace, 0, 0, 0.0, nullptr, nullptr, norm32);
+    RFX_LAUNCH_CHECK();
+    return RFX_OK;
+}
+
+static int scale_launches(const rfx_grad_tensor* tensors, int count, ClipSource from, hipStream_t stream) {
+    GnArgs k;
+    const int piece = piece_of(tensors, count);
+    for (int at = 0;;) {
+        const int taken = gather(tensors, count, at, k, piece, true);
+        if (taken < 0) return taken;
+        if (taken == 0) return no_norm(from.partial, from.norm32, stream);
+        k.clip = from;
+        hipLaunchKernelGGL(grad_scale_kernel, dim3(k.pieces < SC_BLOCKS ? k.pieces : SC_BLOCKS), dim3(SC_THREADS), 0, stream, k);
+        RFX_LAUNCH_CHECK();
+        from.norm32 = nullptr;
+    }
+}
 
 }  // namespace rfx
 
@@ -557,14 +710,17 @@ extern "C" {
 
 size_t rfx_adamw_tensor_bytes(void) { return sizeof(rfx_adamw_tensor); }
 size_t rfx_adamw_group_bytes(void) { return sizeof(rfx_adamw_group); }
-size_t rfx_adamw_workspace_bytes(int count) { return count > 0 ? (size_t)count * sizeof(AwStep) : 0; }
+size_t rfx_adamw_workspace_bytes(int count) {
+    return count > 0 ? ((size_t)count * sizeof(AwStep) + partials(count) * sizeof(double) + 15) / 16 * 16 : 0;
+}
 
-int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_group* groups, int n_groups, const double* clip,
-                   void* workspace, size_t workspace_bytes, rfx_stream stream) {
+int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_group* groups, int n_groups, const rfx_grad_tensor* clip_grads,
+                   double max_norm, float* norm32, void* workspace, size_t workspace_bytes, rfx_stream stream) {
     if (count == 0) return RFX_OK;
     if (!tensors || count < 0 || !groups || n_groups < 1) return RFX_ERR_ARG;
     bool on_device = false;
     unsigned kinds = 0;
+    int64_t bytes = 0;
     for (int i = 0; i < n_groups; ++i)
         if (!group_ok(groups[i])) return RFX_ERR_ARG;
     for (int i = 0; i < count; ++i) {
@@ -572,12 +728,23 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
         if ((tensors[i].n + AW_PIECE - 1) / AW_PIECE > 0x7fffffff) return RFX_ERR_UNSUPPORTED;
         on_device |= tensors[i].step_dev != nullptr;
         kinds |= 1U << kind_of(tensors[i], groups[tensors[i].group]);
+        bytes += tensors[i].n * (2 * elem_bytes(tensors[i].dtype) + (tensors[i].master ? 4 : 0) + (groups[tensors[i].group].state_bits == 8 ? 2 : 8));
     }
-    if (on_device && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < rfx_adamw_workspace_bytes(count))) return RFX_ERR_WORKSPACE;
+    if (clip_grads && (!grads_ok(clip_grads, count) || !(max_norm >= 0.0))) return RFX_ERR_ARG;
+    if ((on_device || clip_grads) && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < rfx_adamw_workspace_bytes(count)))
+        return RFX_ERR_WORKSPACE;
     AwArgs k;
     PrepArgs prep;
     prep.out = (AwStep*)workspace;
-    k.clip = clip;
+    k.clip = ClipSource{};
+    if (clip_grads) {
+        int n = 0;
+        double* at = (double*)((char*)workspace + (size_t)count * sizeof(AwStep));
+        int rc = norm_launches(clip_grads, count, 0, max_norm, at, n, k.clip, as_stream(stream));
+        if (rc == RFX_OK) rc = few(at, n, k.clip, as_stream(stream));
+        if (rc != RFX_OK) return rc;
+        k.clip.norm32 = norm32;
+    }
     for (int kind = 0; kind < 12; ++kind) {
         if (!(kinds >> kind & 1)) continue;
         for (int counted = 0; counted < 2; ++counted) {                    // step counts from the host, then those on the device
@@ -618,24 +785,26 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
                     }
                     --i;                                                   // again, as the first of the next launch
                 }
-                const int rc = adamw_launch(k, counted ? &prep : nullptr, kind, as_stream(stream));
+                const int rc = adamw_launch(k, counted ? &prep : nullptr, kind, bytes >= STREAM_BYTES, as_stream(stream));
                 if (rc != RFX_OK) return rc;
                 used = 0;
                 blocks = 0;
             }
         }
     }
-    return RFX_OK;
+    return no_norm(k.clip.partial, k.clip.norm32, as_stream(stream));
 }
 
 int rfx_adamw_moments(const rfx_moment_tensor* tensors, int count, rfx_stream stream) {
     if (count == 0) return RFX_OK;
     if (!tensors || count < 0) return RFX_ERR_ARG;
+    int64_t bytes = 0;
     for (int i = 0; i < count; ++i) {
         const rfx_moment_tensor& t = tensors[i];
         if (t.n < 0 || (t.n > 0 && (!t.exp_avg || !t.exp_avg_sq || !t.exponents || !t.out_avg || !t.out_avg_sq))) return RFX_ERR_ARG;
         if (((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq | (uintptr_t)t.out_avg | (uintptr_t)t.out_avg_sq) & 3) return RFX_ERR_ARG;
         if ((t.n + AW_PIECE - 1) / AW_PIECE > 0x7fffffff) return RFX_ERR_UNSUPPORTED;
+        bytes += 8 * t.n;                                                  // of the outputs: 332 MB of them 72 us plain, 61 past the caches
     }
     MomArgs k;
     for (int i = 0; i < count;) {
@@ -650,63 +819,50 @@ int rfx_adamw_moments(const rfx_moment_tensor* tensors, int count, rfx_stream st
         }
         if (k.count == 0) break;
         k.first[k.count] = (int32_t)blocks;
-        hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)blocks), dim3(AW_THREADS), 0, as_stream(stream), k);
+        if (bytes >= STREAM_BYTES) hipLaunchKernelGGL(adamw_moments_kernel<true>, dim3((unsigned)blocks), dim3(AW_THREADS), 0, as_stream(stream), k);
+        else hipLaunchKernelGGL(adamw_moments_kernel<false>, dim3((unsigned)blocks), dim3(AW_THREADS), 0, as_stream(stream), k);
         RFX_LAUNCH_CHECK();
     }
     return RFX_OK;
 }
 
-size_t rfx_grad_norm_workspace_bytes(const rfx_grad_tensor* tensors, int count) {
-    if (!grads_ok(tensors, count)) return 0;
-    size_t n = 0;
-    GnArgs k;
-    for (int at = 0; gather(tensors, count, at, k, false) > 0;) n += norm_blocks(k.pieces);
-    return (n ? n : 1) * sizeof(double);
+size_t rfx_grad_norm_workspace_bytes(int count) { return count >= 0 ? partials(count) * sizeof(double) : 0; }
+
+static int norm_args(const rfx_grad_tensor* tensors, int count, int norm_type, double max_norm, const void* workspace, size_t workspace_bytes) {
+    if (!grads_ok(tensors, count) || !(max_norm >= 0.0)) return RFX_ERR_ARG;
+    if (norm_type != 2 && norm_type != 0) return RFX_ERR_UNSUPPORTED;
+    return !workspace || ((uintptr_t)workspace & 7) || workspace_bytes < rfx_grad_norm_workspace_bytes(count) ? RFX_ERR_WORKSPACE : RFX_OK;
 }
 
 int rfx_grad_norm(const rfx_grad_tensor* tensors, int count, int norm_type, double max_norm, double* clip, float* norm32,
                   void* workspace, size_t workspace_bytes, rfx_stream stream) {
-    if (!grads_ok(tensors, count) || !clip || ((uintptr_t)clip & 7) || !(max_norm >= 0.0)) return RFX_ERR_ARG;
-    if (norm_type != 2 && norm_type != 0) return RFX_ERR_UNSUPPORTED;
-    if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < rfx_grad_norm_workspace_bytes(tensors, count)) return RFX_ERR_WORKSPACE;
-    GnArgs k;
-    double* partial = (double*)workspace;
-    int n = 0;
-    for (int at = 0;;) {
-        const int taken = gather(tensors, count, at, k, false);
-        if (taken < 0) return taken;
-        if (taken == 0) break;
-        const int blocks = norm_blocks(k.pieces);
-        k.partial = partial + n;
-        n += blocks;
-        if (norm_type == 2) hipLaunchKernelGGL(grad_norm_kernel<false>, dim3(blocks), dim3(GN_THREADS), 0, as_stream(stream), k);
-        else hipLaunchKernelGGL(grad_norm_kernel<true>, dim3(blocks), dim3(GN_THREADS), 0, as_stream(stream), k);
-        RFX_LAUNCH_CHECK();
-    }
-    if (norm_type == 2) hipLaunchKernelGGL(grad_norm_join_kernel<false>, dim3(1), dim3(GN_THREADS), 0, as_stream(stream), partial, n, max_norm, clip, norm32);
-    else hipLaunchKernelGGL(grad_norm_join_kernel<true>, dim3(1), dim3(GN_THREADS), 0, as_stream(stream), partial, n, max_norm, clip, norm32);
+    if (!clip || ((uintptr_t)clip & 7)) return RFX_ERR_ARG;
+    int rc = norm_args(tensors, count, norm_type, max_norm, workspace, workspace_bytes), n = 0;
+    if (rc != RFX_OK) return rc;
+    ClipSource from;
+    rc = norm_launches(tensors, count, norm_type == 0, max_norm, (double*)workspace, n, from, as_stream(stream));
+    if (rc != RFX_OK) return rc;
+    hipLaunchKernelGGL(grad_norm_join_kernel, dim3(1), dim3(JOIN), 0, as_stream(stream), (const double*)workspace, n, from.max, max_norm, nullptr,
+                       clip, norm32);
     RFX_LAUNCH_CHECK();
     return RFX_OK;
 }
 
-int rfx_grad_clip(const rfx_grad_tensor* tensors, int count, int norm_type, double max_norm, double* clip, float* norm32,
-                  void* workspace, size_t workspace_bytes, rfx_stream stream) {
-    const int rc = rfx_grad_norm(tensors, count, norm_type, max_norm, clip, norm32, workspace, workspace_bytes, stream);
-    return rc == RFX_OK ? rfx_grad_scale(tensors, count, clip, stream) : rc;
+int rfx_grad_scale(const rfx_grad_tensor* tensors, int count, const double* clip, rfx_stream stream) {
+    if (!grads_ok(tensors, count) || !clip || ((uintptr_t)clip & 7)) return RFX_ERR_ARG;
+    return scale_launches(tensors, count, ClipSource{nullptr, clip, 0.0, nullptr, 0, 0}, as_stream(stream));
 }
 
-int rfx_grad_scale(const rfx_grad_tensor* tensors, int count, const double* clip, rfx_stream stream) {
-    if (!grads_ok(tensors, count) || !clip) return RFX_ERR_ARG;
-    GnArgs k;
-    k.clip = clip;
-    for (int at = 0;;) {
-        const int taken = gather(tensors, count, at, k, true);
-        if (taken < 0) return taken;
-        if (taken == 0) break;
-        hipLaunchKernelGGL(grad_scale_kernel, dim3(k.pieces), dim3(GN_THREADS), 0, as_stream(stream), k);
-        RFX_LAUNCH_CHECK();
-    }
-    return RFX_OK;
+int rfx_grad_clip(const rfx_grad_tensor* tensors, int count, int norm_type, double max_norm, float* norm32, void* workspace,
+                  size_t workspace_bytes, rfx_stream stream) {
+    int rc = norm_args(tensors, count, norm_type, max_norm, workspace, workspace_bytes), n = 0;
+    if (rc != RFX_OK) return rc;
+    ClipSource from;
+    rc = norm_launches(tensors, count, norm_type == 0, max_norm, (double*)workspace, n, from, as_stream(stream));
+    if (rc == RFX_OK) rc = few((double*)workspace, n, from, as_stream(stream));
+    if (rc != RFX_OK) return rc;
+    from.norm32 = norm32;
+    return scale_launches(tensors, count, from, as_stream(stream));
 }
 
 }  // extern "C"

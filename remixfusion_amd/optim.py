@@ -224,7 +224,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     lib, rows, n, kind = _lib.load(), _grad_rows(flat), len(flat), 2 if norm_type == 2.0 else 0
     with _on(dev.index), torch.no_grad():
         stream = _lib.stream_ptr(dev)
-        ws_bytes = lib.rfx_grad_norm_workspace_bytes(rows, n)
+        ws_bytes = lib.rfx_grad_norm_workspace_bytes(n)
         ws = torch.empty(2 + ws_bytes // 8, dtype=torch.float64, device=dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
         clip = ws.data_ptr()

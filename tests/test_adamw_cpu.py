@@ -106,10 +106,11 @@ def _group(**kw):
     return g
 
 
-def _call(t, g, count=1, groups=1, ws=None, ws_bytes=0):
+def _call(t, g, count=1, groups=1, ws=None, ws_bytes=0, clip=None, limit=0.0):
     arr = (L.AdamwTensor * 1)(t) if t is not None else None
     garr = (L.AdamwGroup * 1)(g) if g is not None else None
-    return L.load().rfx_adamw_step(C.addressof(arr) if arr else None, count, C.addressof(garr) if garr else None, groups, None, ws, ws_bytes, None)
+    return L.load().rfx_adamw_step(C.addressof(arr) if arr else None, count, C.addressof(garr) if garr else None, groups,
+                                 C.addressof(clip) if clip else None, limit, None, ws, ws_bytes, None)
 
 
 def test_struct_layouts_match_the_library():
@@ -140,9 +141,15 @@ def test_adamw_step_refusals_and_empty_calls():
     assert _call(_tensor(n=0, param=None), _group()) == 0                               # no elements: nothing to launch
     assert _call(_tensor(n=1 << 52), _group()) == -3
     lib = L.load()
-    assert lib.rfx_adamw_workspace_bytes(0) == 0 and lib.rfx_adamw_workspace_bytes(-3) == 0 and lib.rfx_adamw_workspace_bytes(3) == 48
-    for ws, n in ((None, 0), (A, 15), (A + 8, 64)):                                     # a count on the device needs the workspace
+    assert lib.rfx_adamw_workspace_bytes(0) == 0 and lib.rfx_adamw_workspace_bytes(-3) == 0 and lib.rfx_adamw_workspace_bytes(3) >= 48
+    grads = (L.GradTensor * 1)(L.GradTensor(A + 4096, 8, 0, 0))
+    for ws, n in ((None, 0), (A, 15), (A + 8, 1 << 16)):                                # a count on the device, or a norm, needs the workspace
         assert _call(_tensor(step_dev=A), _group(), ws=ws, ws_bytes=n) == -4
+        assert _call(_tensor(), _group(), ws=ws, ws_bytes=n, clip=grads, limit=1.0) == -4
+    for limit in (-1.0, math.nan):
+        assert _call(_tensor(), _group(), ws=A, ws_bytes=1 << 16, clip=grads, limit=limit) == -1
+    grads[0].dtype = 7
+    assert _call(_tensor(), _group(), ws=A, ws_bytes=1 << 16, clip=grads, limit=1.0) == -1
 
 
 def test_norm_scale_and_moments_refusals():
@@ -159,12 +166,14 @@ def test_norm_scale_and_moments_refusals():
 
     for kw in (dict(grad=None), dict(n=-1), dict(dtype=3), dict(grad=A + 2), dict(dtype=2, grad=A + 1)):
         assert norm(grads(**kw)) == -1 and lib.rfx_grad_scale(C.addressof(grads(**kw)), 1, A, None) == -1
-        assert lib.rfx_grad_norm_workspace_bytes(C.addressof(grads(**kw)), 1) == 0
+        assert lib.rfx_grad_clip(C.addressof(grads(**kw)), 1, 2, 1.0, None, A, 1 << 16, None) == -1
     ok = grads()
     assert norm(None) == -1 and norm(ok, -1) == -1 and norm(ok, clip=None) == -1 and norm(ok, clip=A + 4) == -1
     assert norm(ok, limit=-1.0) == -1 and norm(ok, limit=math.nan) == -1 and norm(ok, kind=1) == -3
     assert norm(ok, ws=None) == -4 and norm(ok, ws_bytes=7) == -4 and norm(ok, ws=A + 4) == -4
-    assert lib.rfx_grad_scale(C.addressof(ok), 1, None, None) == -1 and lib.rfx_grad_scale(None, 0, A, None) == 0
+    assert lib.rfx_grad_clip(C.addressof(ok), 1, 2, 1.0, None, A, 7, None) == -4 and lib.rfx_grad_clip(C.addressof(ok), 1, 3, 1.0, None, A, 1 << 16, None) == -3
+    assert lib.rfx_grad_norm_workspace_bytes(-1) == 0 and lib.rfx_grad_norm_workspace_bytes(1) >= 2048
+    assert lib.rfx_grad_scale(C.addressof(ok), 1, None, None) == -1 and lib.rfx_grad_scale(C.addressof(ok), 1, A + 4, None) == -1 and lib.rfx_grad_scale(None, 0, A, None) == 0
     m = L.MomentTensor(A, A, A, A, A, 8)
     for k in ("exp_avg", "exp_avg_sq", "exponents", "out_avg", "out_avg_sq"):
         bad = (L.MomentTensor * 1)(m)
