@@ -704,7 +704,7 @@ def ShardedPipeline(config: Dict, dist, rank: int, world: int, device: str = "cu
                         broadcast_(dist, prm.data, 0)
                 for opt in (self.slam.map_optimizer, self.slam.rba_optimizer):
                     for st in opt.state.values():
-                        for k in ("exp_avg", "exp_avg_sq"):
+                        for k in ("exp_avg", "exp_avg_sq", "exponents", "master"):
                             if k in st:
                                 broadcast_(dist, st[k], 0)
 

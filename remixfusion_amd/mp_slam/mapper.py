@@ -324,6 +324,8 @@ class Mapper:
                 mode = str(self.config["mapping"].get("shard_field", "auto"))
                 if mode not in ("auto", "levels", "replicas"):
                     raise _lib.RfxError(f"mapping.shard_field: {mode!r}")
+                if mode == "auto" and not hasattr(self.map_optimizer, "slices"):
+                    mode = "replicas"       # (AdamW steps whole tensors only)
                 if mode == "auto":          # the cheaper of the two by the time model of dist.choose_field_mode
                     from ..dist import choose_field_mode
                     m, tr = self.config["mapping"], self.config["training"]

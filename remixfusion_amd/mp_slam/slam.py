@@ -198,13 +198,26 @@ class SLAM:
         return poses
 
     def create_optimizer(self):
-        """two Adams: map (decoder wd 1e-6, hash eps 1e-15) and pose MLP (reference :271-286)."""
+        """two Adams: map (decoder wd 1e-6, hash eps 1e-15) and pose MLP (reference :271-286).  mapping.optimizer "adamw" steps both
+        with decoupled decay, "adamw8bit" also holds the hash table's moments -- nearly all of an optimizer's memory -- in one byte each;
+        mapping.grad_clip then limits the global norm of each optimizer's gradients (remixfusion_amd/optim.py::AdamW)."""
         m = self.config["mapping"]
         trainable = [
             {"params": list(self.model.decoder_res.parameters()), "weight_decay": 1e-6, "lr": m["lr_decoder"]},
             {"params": list(self.model.embed_res_fn.parameters()), "eps": 1e-15, "lr": m["lr_embed_res"]},
         ]
         rba = [{"params": list(self.model.rba.parameters()), "weight_decay": 1e-6, "eps": 1e-15, "lr": m["lr_pose"]}]
+        kind, clip = m.get("optimizer", "adam"), m.get("grad_clip")
+        if kind not in ("adam", "adamw", "adamw8bit"):
+            raise ValueError(f"mapping.optimizer is adam, adamw or adamw8bit: {kind!r}")
+        if kind != "adam":
+            from ..optim import AdamW
+            trainable[1].update(weight_decay=0.0, state_bits=8 if kind == "adamw8bit" else 32)      # (AdamW's own default decays)
+            self.map_optimizer = AdamW(trainable, betas=(0.9, 0.99), max_grad_norm=clip)
+            self.rba_optimizer = AdamW(rba, betas=(0.9, 0.99), max_grad_norm=clip)
+            return
+        if clip is not None:
+            raise ValueError("mapping.grad_clip needs mapping.optimizer adamw or adamw8bit")
         # same Adam as the reference (torch.optim.Adam, betas (0.9, 0.99)); on the device its step is one librfx launch
         # over all tensors of the optimizer (remixfusion_amd/optim.py); mapping.fused_adam=False keeps torch's own step
         if self.config["mapping"].get("fused_adam", True) and all(p.is_cuda for g in trainable + rba for p in g["params"]):
