@@ -41,7 +41,7 @@ class Adam(torch.optim.Adam):
         if self.slices and not all(p.is_cuda for p in self.slices):
             raise _lib.RfxError("a sliced Adam step needs device parameters (there is no CPU path)")
         for g in self.param_groups:
-            if g.get("amsgrad") or g.get("maximize") or g.get("capturable") or g.get("differentiable"):
+            if g.get("amsgrad") or g.get("maximize") or g.get("capturable") or g.get("differentiable") or g.get("decoupled_weight_decay"):
                 return False
             if isinstance(g["lr"], torch.Tensor):
                 return False

@@ -738,3 +738,15 @@ def test_closure_and_zero_sized():
     only = AdamW([e])
     only.step()
     assert float(clip_grad_norm_([e], 1.0)) == 0.0 and [t.shape for t in only.moments()[0]] == [(0, 3)]
+
+
+def test_adam_with_decoupled_decay_is_not_stepped_as_l2():
+    """optim.Adam's native step folds the decay into the gradient: the decoupled kind takes torch's step"""
+    from remixfusion_amd.optim import Adam
+    p, q = (torch.nn.Parameter(torch.linspace(-1, 1, 100, device="cuda")) for _ in range(2))
+    ours = Adam([p], lr=0.1, weight_decay=0.5, decoupled_weight_decay=True)
+    ref = torch.optim.Adam([q], lr=0.1, weight_decay=0.5, decoupled_weight_decay=True)
+    for _ in range(2):
+        p.grad = q.grad = torch.full((100,), 0.25, device="cuda")
+        ours.step(); ref.step()
+    assert float((p - q).detach().abs().max()) <= 1e-6
