@@ -280,6 +280,10 @@ template <bool FULL> __device__ __forceinline__ void adamw8_run(Run8& r, const A
     r.e1 = run_exponent<1>(wave_max(h1));
     r.e2 = run_exponent<2>(wave_max(h2));
     const double i1 = pow2(-112 - r.e1), i2 = pow2(-96 - 2 * r.e2);
+    // the root is taken of v 2^(2 half), which no fp32 overflows and next to none underflows: squares of fp32 numbers do both
+    const int half = r.e2 < -50 ? 100 : 50 - r.e2;
+    const double up = pow2(2 * half);
+    const float down = s.inv_bc2 * __uint_as_float((uint32_t)(127 - half) << 23);
     r.cm = r.cv = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -291,11 +295,9 @@ template <bool FULL> __device__ __forceinline__ void adamw8_run(Run8& r, const A
         cv = cv > some ? cv : some;
         r.cm |= (cm | ((uint32_t)__double2hiint(m[j]) >> 24 & 128U)) << (8 * j);
         r.cv |= cv << (8 * j);
-        // fp32, the chip's own root and reciprocal (an ulp each, under 16 u of the update all told).  They take subnormals for 0: a
-        // second moment under 2^-126 counts as that much
-        const float root = __builtin_amdgcn_sqrtf(fmaxf((float)v[j], 1.17549435e-38f));
-        const float d = madd(root, s.inv_bc2, a.eps);
-        r.x[j] -= madd(s.lr_wd, r.x[j], s.step_size * ((float)m[j] * __builtin_amdgcn_rcpf(d)));
+        // fp32, the chip's own root and reciprocal: an ulp each, under 16 u of the update all told
+        const float d = madd(__builtin_amdgcn_sqrtf((float)(v[j] * up)), down, a.eps);
+        r.x[j] -= madd(s.lr_wd, r.x[j], s.step_size * (float)m[j] * __builtin_amdgcn_rcpf(d));
     }
 }
 

@@ -290,6 +290,41 @@ def test_eight_bits_over_the_whole_range():
         assert bool(torch.isfinite(p).all()) and float(p.detach().abs().max()) <= 1e-3 * (it + 1) * 40     # m without its v would be m / eps
 
 
+@pytest.mark.parametrize("eps", [1e-15, 1e-8])
+def test_eight_bit_states_of_any_bytes(eps):
+    """every code under every exponent, moments that no run of steps leaves (m without v, roots beyond fp32's range): the step is the
+    formula's.  m / eps may be of any size, so the tolerance is relative to the update."""
+    from remixfusion_amd.optim import AdamW
+    rng = np.random.default_rng(77)
+    n = 256 * 600 + 131
+    rows = -(-n // 256)
+    cm, cv = rng.integers(0, 256, n, dtype=np.uint8), rng.integers(0, 256, n, dtype=np.uint8)
+    cv[rng.random(n) < 0.2] = 0
+    e1 = rng.integers(-127, 100, rows).astype(np.int8)
+    e2 = np.clip(e1 + rng.integers(-3, 4, rows), -127, 127).astype(np.int8)
+    g = np.where(rng.random(n) < 0.5, 0.0, rng.standard_normal(n) * np.repeat(2.0 ** np.clip(e1.astype(float), -120, 100), 256)[:n]).astype(np.float32)
+    p = torch.nn.Parameter(torch.from_numpy(rng.standard_normal(n).astype(np.float32)).cuda())
+    ref = Ref(p.detach().cpu().numpy(), 8, 0, 13)
+    ref.k, ref.m, ref.v = 30, decode(cm, e1, 15), decode(cv, e2, 31)
+    opt = AdamW([p], lr=1e-3, betas=(0.9, 0.99), eps=eps, weight_decay=0.01, state_bits=8, seed=13)
+    state = {"step": torch.tensor(30.0), "exp_avg": torch.from_numpy(cm).cuda(), "exp_avg_sq": torch.from_numpy(cv).cuda(),
+             "exponents": torch.from_numpy(np.stack([e1, e2])).cuda()}
+    opt.load_state_dict({"state": {0: state}, "param_groups": opt.state_dict()["param_groups"]})
+    p.grad = torch.from_numpy(g).cuda()
+    old = ref.p.copy()
+    opt.step()
+    tp, _, _ = ref.step(g, 1e-3, (0.9, 0.99), eps, 0.01)
+    _check_code(opt.state[p], ref, eps)
+    # m is formed in fp64 here (4 u of each of its terms do not arise), rounded to fp32 once; what fp32 cannot hold is inf on the way out
+    up = np.abs(ref.p - old * (1 - 1e-5))
+    tol = U * (np.abs(old) + np.abs(ref.p)) + 16 * U * up + 2.0 ** -140
+    fits = np.abs(ref.p) < 1e37
+    got = p.detach().double().cpu().numpy()
+    assert int((~fits).sum()) < n // 2
+    bad = fits & ~(np.abs(got - ref.p) <= tol)
+    assert not bad.any(), [(int(i), got[i], ref.p[i], tol[i]) for i in np.flatnonzero(bad)[:4]]
+
+
 def test_rounding_is_unbiased_and_an_average_keeps_moving():
     """A code's expectation is the value itself: over 4096 seeds the mean is within 6 sigma of it, sigma <= step / 2 / sqrt(4096).
     And v of a constant gradient grows to g^2 although one step's change (1/1000) is far below the format's (1/8): with
