@@ -4,14 +4,16 @@
 // (8-bit moments) of HBM traffic and some dozens of vector instructions, so the bytes are the bound and the instructions are
 // what has to stay under them.  All tensors of a kind (type, state, master copy) go into one launch: their descriptors travel in
 // the kernel's arguments (no table in device memory that a later call could overwrite under a running kernel or a captured one),
-// every tensor is cut into pieces of PIECE elements, and a block finds its tensor by bisection over the first pieces.
+// every tensor is cut into pieces of AW_PIECE elements, and a block finds its tensor by bisection over the first pieces.
 #include "rfx_common.h"
 #include <math.h>
 
 namespace rfx {
 
 constexpr int AW_THREADS = 256;
-constexpr int AW_PIECE = 4096;          // elements per block
+// Elements per block: four a thread, one run of the 8-bit form a wave.  Small blocks fill the chip early and leave no tail: against 4096
+// elements, 135 000 parameters in 8 bits step in 5 us instead of 9, and 41.5 million in 32 bits in 194 us instead of 206.
+constexpr int AW_PIECE = AW_THREADS * 4;
 constexpr int AW_TENSORS = 48;          // descriptors per launch: the kernel's arguments stay under 4 KB
 constexpr int AW_GROUPS = 8;
 constexpr int AW_RUN = RFX_ADAMW_BLOCK;
@@ -179,26 +181,26 @@ __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(const AwArgs k) {
     float* v = (float*)t.v + base;
     float* w = MASTER ? t.w + base : nullptr;
     const bool vec = ((((uintptr_t)p | (uintptr_t)g) & (4 * sizeof(T) - 1)) | (((uintptr_t)m | (uintptr_t)v | (uintptr_t)w) & 15)) == 0;
-    int done = 0;
-    if (vec) {
-        done = len & ~3;
-        for (int i = threadIdx.x * 4; i < done; i += AW_THREADS * 4) {
-            f4 x = MASTER ? load4<STREAM>(w + i) : load4<STREAM>(p + i);
-            const f4 gg = load4<STREAM>(g + i);
-            f4 mm = load4<STREAM>(m + i), vv = load4<STREAM>(v + i);
+    int i = threadIdx.x * 4;
+    if (vec && i + 4 <= len) {
+        f4 x = MASTER ? load4<STREAM>(w + i) : load4<STREAM>(p + i);
+        const f4 gg = load4<STREAM>(g + i);
+        f4 mm = load4<STREAM>(m + i), vv = load4<STREAM>(v + i);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float xj = x[j], mj = mm[j], vj = vv[j];
-                adamw_one(xj, gg[j], mj, vj, a, s, c);
-                x[j] = xj; mm[j] = mj; vv[j] = vj;
-            }
-            store4<STREAM>(p + i, x);
-            if (MASTER) store4<STREAM>(w + i, x);
-            store4<STREAM>(m + i, mm);
-            store4<STREAM>(v + i, vv);
+        for (int j = 0; j < 4; ++j) {
+            float xj = x[j], mj = mm[j], vj = vv[j];
+            adamw_one(xj, gg[j], mj, vj, a, s, c);
+            x[j] = xj; mm[j] = mj; vv[j] = vj;
         }
+        store4<STREAM>(p + i, x);
+        if (MASTER) store4<STREAM>(w + i, x);
+        store4<STREAM>(m + i, mm);
+        store4<STREAM>(v + i, vv);
+        return;
     }
-    for (int i = done + threadIdx.x; i < len; i += AW_THREADS) {
+    int step = 1, end = i + 4 < len ? i + 4 : len;                         // the last elements of a tensor: those of this lane
+    if (!vec) { i = threadIdx.x; step = AW_THREADS; end = len; }           // no vector load fits: neighbours to neighbouring lanes
+    for (; i < end; i += step) {
         float x = MASTER ? w[i] : (float)p[i], mm = m[i], vv = v[i];
         adamw_one(x, (float)g[i], mm, vv, a, s, c);
         p[i] = (T)x;
@@ -323,38 +325,25 @@ __global__ __launch_bounds__(AW_THREADS) void adamw8_kernel(const AwArgs k) {
     int8_t* e1 = t.e + run0;
     int8_t* e2 = t.e + runs + run0;
     const bool vec = ((((uintptr_t)p | (uintptr_t)g) & (4 * sizeof(T) - 1)) | ((uintptr_t)w & 15)) == 0;
+    const int run = wave, i = run * AW_RUN + lane * 4;
+    const uint32_t run_key = mix32(key + (uint32_t)run);
+    Run8 x;
     if (len == AW_PIECE && vec) {
-        constexpr int MINE = AW_PIECE / AW_RUN / (AW_THREADS / 64);        // runs of a wave, the next one's loads on their way while one is stepped
-        const auto load = [&](int r) {
-            const int i = (wave + r * (AW_THREADS / 64)) * AW_RUN + lane * 4;
-            Run8 x;
-            x.x = MASTER ? load4<STREAM>(w + i) : load4<STREAM>(p + i);
-            x.g = load4<STREAM>(g + i);
-            x.cm = *reinterpret_cast<const uint32_t*>(m + i);
-            x.cv = *reinterpret_cast<const uint32_t*>(v + i);
-            x.e1 = e1[wave + r * (AW_THREADS / 64)];
-            x.e2 = e2[wave + r * (AW_THREADS / 64)];
-            return x;
-        };
-        Run8 next = load(0);
-#pragma unroll
-        for (int r = 0; r < MINE; ++r) {
-            Run8 x = next;
-            if (r + 1 < MINE) next = load(r + 1);
-            const int run = wave + r * (AW_THREADS / 64), i = run * AW_RUN + lane * 4;
-            adamw8_run<true>(x, a, s, c, mix32(key + (uint32_t)run), lane, 4);
-            store4<STREAM>(p + i, x.x);
-            if (MASTER) store4<STREAM>(w + i, x.x);
-            *reinterpret_cast<uint32_t*>(m + i) = x.cm;
-            *reinterpret_cast<uint32_t*>(v + i) = x.cv;
-            if (lane == 0) { e1[run] = (int8_t)x.e1; e2[run] = (int8_t)x.e2; }
-        }
-        return;
-    }
-    for (int run = wave; run * AW_RUN < len; run += AW_THREADS / 64) {     // a tensor's last piece, or one that vector loads do not fit
-        const int i = run * AW_RUN + lane * 4;
+        x.x = MASTER ? load4<STREAM>(w + i) : load4<STREAM>(p + i);
+        x.g = load4<STREAM>(g + i);
+        x.cm = *reinterpret_cast<const uint32_t*>(m + i);
+        x.cv = *reinterpret_cast<const uint32_t*>(v + i);
+        x.e1 = e1[run];
+        x.e2 = e2[run];
+        adamw8_run<true>(x, a, s, c, run_key, lane, 4);
+        store4<STREAM>(p + i, x.x);
+        if (MASTER) store4<STREAM>(w + i, x.x);
+        *reinterpret_cast<uint32_t*>(m + i) = x.cm;
+        *reinterpret_cast<uint32_t*>(v + i) = x.cv;
+    } else {                                                               // a tensor's last piece, or one that vector loads do not fit
+        if (run * AW_RUN >= len) return;
         const int have = len - i < 0 ? 0 : len - i > 4 ? 4 : len - i;      // elements of this lane
-        Run8 x{};
+        x = Run8{};
         for (int j = 0; j < have; ++j) {
             x.x[j] = MASTER ? w[i + j] : (float)p[i + j];
             x.g[j] = (float)g[i + j];
@@ -363,15 +352,15 @@ __global__ __launch_bounds__(AW_THREADS) void adamw8_kernel(const AwArgs k) {
         }
         x.e1 = e1[run];
         x.e2 = e2[run];
-        adamw8_run<false>(x, a, s, c, mix32(key + (uint32_t)run), lane, have);
+        adamw8_run<false>(x, a, s, c, run_key, lane, have);
         for (int j = 0; j < have; ++j) {
             p[i + j] = (T)x.x[j];
             if (MASTER) w[i + j] = x.x[j];
             m[i + j] = (uint8_t)(x.cm >> (8 * j));
             v[i + j] = (uint8_t)(x.cv >> (8 * j));
         }
-        if (lane == 0) { e1[run] = (int8_t)x.e1; e2[run] = (int8_t)x.e2; }
     }
+    if (lane == 0) { e1[run] = (int8_t)x.e1; e2[run] = (int8_t)x.e2; }
 }
 
 // step counts on the device (captured calls): raise them and derive what they decide, one thread a tensor
@@ -413,7 +402,8 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_moments_kernel(const MomArgs
     float* om = t.out_avg + base;
     float* ov = t.out_avg_sq + base;
     const bool vec = (((uintptr_t)om | (uintptr_t)ov) & 15) == 0;
-    for (int i = threadIdx.x * 4; i < len; i += AW_THREADS * 4) {
+    const int i = threadIdx.x * 4;
+    if (i < len) {
         const int64_t run = piece * (AW_PIECE / AW_RUN) + i / AW_RUN;
         const int have = len - i > 4 ? 4 : len - i;
         const double s1 = scale_m(t.exponents[run]), s2 = scale_v(t.exponents[runs + run]);
@@ -494,15 +484,13 @@ __global__ __launch_bounds__(GN_THREADS) void grad_norm_kernel(const GnArgs k) {
     if (threadIdx.x == 0) k.partial[blockIdx.x] = r;
 }
 
-// many partial results (of several launches) to one, or to the norm and its factor
-__global__ __launch_bounds__(JOIN) void grad_norm_join_kernel(const double* partial, int n, int max, double max_norm, double* one, double* clip,
-                                                              float* norm32) {
+// partial results to the norm and its factor
+__global__ __launch_bounds__(JOIN) void grad_norm_join_kernel(const double* partial, int n, int max, double max_norm, double* clip, float* norm32) {
     __shared__ double lds[JOIN / 64];
     double x = 0.0;
     for (int i = threadIdx.x; i < n; i += JOIN) x = max ? larger(x, partial[i]) : x + partial[i];
     x = block_join<JOIN>(x, max != 0, lds);
     if (threadIdx.x != 0) return;
-    if (one) { *one = x; return; }
     const double norm = max ? x : sqrt(x);
     if (clip) {
         clip[0] = norm;
@@ -543,9 +531,10 @@ static int elem_bytes(int dtype) { return dtype == RFX_F32 ? 4 : 2; }
 // Measured, us a step (plain loads and stores / past the caches): 26 MB of fp32 tensors stepped again and again 9.5 / 11.6, 64 MB 19.6 / 25,
 // 128 MB 46 / 43, 665 MB 222 / 204; behind other work on 256 MB, as in a training loop, 16 MB 13.8 / 8.1, 64 MB 44 / 26, 128 MB 68 / 44.
 constexpr int64_t STREAM_BYTES = 64 << 20;
+static int64_t pieces_of(int64_t n) { return (n + AW_PIECE - 1) / AW_PIECE; }
 
 // one launch of the tensors gathered in `k`; dev: their scalars' place in the workspace (step counts on the device)
-static int adamw_launch(AwArgs& k, PrepArgs* prep, int kind, bool stream_past, hipStream_t stream) {
+static int adamw_launch(AwArgs& k, PrepArgs* prep, int kind, bool past, hipStream_t stream) {
     if (k.count == 0) return RFX_OK;
     if (prep) {
         prep->count = k.count;
@@ -559,7 +548,7 @@ static int adamw_launch(AwArgs& k, PrepArgs* prep, int kind, bool stream_past, h
         return RFX_OK;
     }
     const void* kernel = nullptr;
-    const auto pick = [&](auto plain, auto streaming) { kernel = stream_past ? (const void*)streaming : (const void*)plain; };
+    const auto pick = [&](auto plain, auto streaming) { kernel = past ? (const void*)streaming : (const void*)plain; };
     switch (kind) {
         case 0: pick(adamw32_kernel<RFX_F32, false, false>, adamw32_kernel<RFX_F32, false, true>); break;
         case 1: pick(adamw32_kernel<RFX_BF16, false, false>, adamw32_kernel<RFX_BF16, false, true>); break;
@@ -649,7 +638,12 @@ static int piece_of(const rfx_grad_tensor* t, int count) {
     return (int)(piece < GN_LEAST ? GN_LEAST : piece > GN_MOST ? GN_MOST : piece);
 }
 
-static size_t partials(int count) { return (size_t)JOIN * ((count + GN_TENSORS - 1) / GN_TENSORS) + 1; }
+// Blocks of the 8-bit step from which the partial results are joined in a launch of their own.  A clipped step, us (every block / a launch):
+// 0.1 million parameters 9.2 / 11.5, 4 million 23.7 / 23.4, 16 million 70 / 65, 40 million 159 / 143.  The 32-bit step waits for memory
+// anyway: 11.7 / 12.9, 28.0 / 28.6, 90.1 / 90.6, 197.4 / 198.0.
+constexpr int64_t JOIN_BLOCKS = 4096;
+
+static size_t partials(int count) { return (size_t)JOIN * ((count + GN_TENSORS - 1) / GN_TENSORS) + 2; }
 
 // partial results of the norm; `from`: how a kernel finds the factor in them
 static int norm_launches(const rfx_grad_tensor* tensors, int count, int max, double max_norm, double* workspace, int& n, ClipSource& from,
@@ -672,20 +666,20 @@ static int norm_launches(const rfx_grad_tensor* tensors, int count, int max, dou
     return RFX_OK;
 }
 
-// ... and at most as many of them as a kernel's block joins by itself
-static int few(double* workspace, int n, ClipSource& from, hipStream_t stream) {
-    if (n <= JOIN) return RFX_OK;                                          // (none: no element, and nothing that would ask)
-    hipLaunchKernelGGL(grad_norm_join_kernel, dim3(1), dim3(JOIN), 0, stream, workspace, n, from.max, 0.0, workspace + n, nullptr, nullptr);
+// ... joined beforehand where there are more than a block joins by itself, or many blocks that would
+static int join(double* workspace, int n, int64_t blocks, float* norm32, ClipSource& from, hipStream_t stream) {
+    from.norm32 = norm32;
+    if (n <= JOIN && blocks <= JOIN_BLOCKS) return RFX_OK;
+    hipLaunchKernelGGL(grad_norm_join_kernel, dim3(1), dim3(JOIN), 0, stream, workspace, n, from.max, from.max_norm, workspace + n, norm32);
     RFX_LAUNCH_CHECK();
-    from.partial = workspace + n;
-    from.n = 1;
+    from = ClipSource{workspace, workspace + n, 0.0, nullptr, 0, 0};
     return RFX_OK;
 }
 
 // the norm of no element at all, which no other launch of the call has written
 static int no_norm(const double* workspace, float* norm32, hipStream_t stream) {
     if (!norm32) return RFX_OK;
-    hipLaunchKernelGGL(grad_norm_join_kernel, dim3(1), dim3(JOIN), 0, stream, workspace, 0, 0, 0.0, nullptr, nullptr, norm32);
+    hipLaunchKernelGGL(grad_norm_join_kernel, dim3(1), dim3(JOIN), 0, stream, workspace, 0, 0, 0.0, nullptr, norm32);
     RFX_LAUNCH_CHECK();
     return RFX_OK;
 }
@@ -722,19 +716,21 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
     if (!tensors || count < 0 || !groups || n_groups < 1) return RFX_ERR_ARG;
     bool on_device = false;
     unsigned kinds = 0;
-    int64_t bytes = 0;
+    int64_t bytes = 0, blocks8 = 0;
     for (int i = 0; i < n_groups; ++i)
         if (!group_ok(groups[i])) return RFX_ERR_ARG;
     for (int i = 0; i < count; ++i) {
         if (!tensor_ok(tensors[i], groups, n_groups)) return RFX_ERR_ARG;
-        if ((tensors[i].n + AW_PIECE - 1) / AW_PIECE > 0x7fffffff) return RFX_ERR_UNSUPPORTED;
+        if (pieces_of(tensors[i].n) > 0x7fffffff) return RFX_ERR_UNSUPPORTED;
         on_device |= tensors[i].step_dev != nullptr;
         kinds |= 1U << kind_of(tensors[i], groups[tensors[i].group]);
         bytes += tensors[i].n * (2 * elem_bytes(tensors[i].dtype) + (tensors[i].master ? 4 : 0) + (groups[tensors[i].group].state_bits == 8 ? 2 : 8));
+        if (groups[tensors[i].group].state_bits == 8) blocks8 += pieces_of(tensors[i].n);
     }
     if (clip_grads && (!grads_ok(clip_grads, count) || !(max_norm >= 0.0))) return RFX_ERR_ARG;
     if ((on_device || clip_grads) && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < rfx_adamw_workspace_bytes(count)))
         return RFX_ERR_WORKSPACE;
+    const bool past = bytes >= STREAM_BYTES;
     AwArgs k;
     PrepArgs prep;
     prep.out = (AwStep*)workspace;
@@ -743,9 +739,8 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
         int n = 0;
         double* at = (double*)((char*)workspace + (size_t)count * sizeof(AwStep));
         int rc = norm_launches(clip_grads, count, 0, max_norm, at, n, k.clip, as_stream(stream));
-        if (rc == RFX_OK) rc = few(at, n, k.clip, as_stream(stream));
+        if (rc == RFX_OK) rc = join(at, n, blocks8, norm32, k.clip, as_stream(stream));
         if (rc != RFX_OK) return rc;
-        k.clip.norm32 = norm32;
     }
     for (int kind = 0; kind < 12; ++kind) {
         if (!(kinds >> kind & 1)) continue;
@@ -760,7 +755,7 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
                     const rfx_adamw_tensor& t = tensors[i];
                     if (kind_of(t, groups[t.group]) != kind || (t.step_dev != nullptr) != (counted != 0)) continue;
                     if (t.n == 0 && !counted) continue;
-                    const int64_t pieces = (t.n + AW_PIECE - 1) / AW_PIECE;
+                    const int64_t pieces = pieces_of(t.n);
                     int gi = 0;
                     while (gi < used && group_at[gi] != t.group) ++gi;
                     bool full = k.count == AW_TENSORS || gi == AW_GROUPS || blocks + pieces > 0x7fffffff;
@@ -787,7 +782,7 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
                     }
                     --i;                                                   // again, as the first of the next launch
                 }
-                const int rc = adamw_launch(k, counted ? &prep : nullptr, kind, bytes >= STREAM_BYTES, as_stream(stream));
+                const int rc = adamw_launch(k, counted ? &prep : nullptr, kind, past, as_stream(stream));
                 if (rc != RFX_OK) return rc;
                 used = 0;
                 blocks = 0;
@@ -805,7 +800,7 @@ int rfx_adamw_moments(const rfx_moment_tensor* tensors, int count, rfx_stream st
         const rfx_moment_tensor& t = tensors[i];
         if (t.n < 0 || (t.n > 0 && (!t.exp_avg || !t.exp_avg_sq || !t.exponents || !t.out_avg || !t.out_avg_sq))) return RFX_ERR_ARG;
         if (((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq | (uintptr_t)t.out_avg | (uintptr_t)t.out_avg_sq) & 3) return RFX_ERR_ARG;
-        if ((t.n + AW_PIECE - 1) / AW_PIECE > 0x7fffffff) return RFX_ERR_UNSUPPORTED;
+        if (pieces_of(t.n) > 0x7fffffff) return RFX_ERR_UNSUPPORTED;
         bytes += 8 * t.n;                                                  // of the outputs: 332 MB of them 72 us plain, 61 past the caches
     }
     MomArgs k;
@@ -813,7 +808,7 @@ int rfx_adamw_moments(const rfx_moment_tensor* tensors, int count, rfx_stream st
         int64_t blocks = 0;
         for (k.count = 0; i < count && k.count < AW_TENSORS; ++i) {
             if (tensors[i].n == 0) continue;
-            const int64_t pieces = (tensors[i].n + AW_PIECE - 1) / AW_PIECE;
+            const int64_t pieces = pieces_of(tensors[i].n);
             if (blocks + pieces > 0x7fffffff) break;
             k.t[k.count] = tensors[i];
             k.first[k.count++] = (int32_t)blocks;
@@ -821,8 +816,8 @@ int rfx_adamw_moments(const rfx_moment_tensor* tensors, int count, rfx_stream st
         }
         if (k.count == 0) break;
         k.first[k.count] = (int32_t)blocks;
-        if (bytes >= STREAM_BYTES) hipLaunchKernelGGL(adamw_moments_kernel<true>, dim3((unsigned)blocks), dim3(AW_THREADS), 0, as_stream(stream), k);
-        else hipLaunchKernelGGL(adamw_moments_kernel<false>, dim3((unsigned)blocks), dim3(AW_THREADS), 0, as_stream(stream), k);
+        const auto kernel = bytes >= STREAM_BYTES ? adamw_moments_kernel<true> : adamw_moments_kernel<false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(AW_THREADS), 0, as_stream(stream), k);
         RFX_LAUNCH_CHECK();
     }
     return RFX_OK;
@@ -844,8 +839,8 @@ int rfx_grad_norm(const rfx_grad_tensor* tensors, int count, int norm_type, doub
     ClipSource from;
     rc = norm_launches(tensors, count, norm_type == 0, max_norm, (double*)workspace, n, from, as_stream(stream));
     if (rc != RFX_OK) return rc;
-    hipLaunchKernelGGL(grad_norm_join_kernel, dim3(1), dim3(JOIN), 0, as_stream(stream), (const double*)workspace, n, from.max, max_norm, nullptr,
-                       clip, norm32);
+    hipLaunchKernelGGL(grad_norm_join_kernel, dim3(1), dim3(JOIN), 0, as_stream(stream), (const double*)workspace, n, from.max, max_norm, clip,
+                       norm32);
     RFX_LAUNCH_CHECK();
     return RFX_OK;
 }
@@ -861,9 +856,8 @@ int rfx_grad_clip(const rfx_grad_tensor* tensors, int count, int norm_type, doub
     if (rc != RFX_OK) return rc;
     ClipSource from;
     rc = norm_launches(tensors, count, norm_type == 0, max_norm, (double*)workspace, n, from, as_stream(stream));
-    if (rc == RFX_OK) rc = few((double*)workspace, n, from, as_stream(stream));
+    if (rc == RFX_OK) rc = join((double*)workspace, n, 0, norm32, from, as_stream(stream));
     if (rc != RFX_OK) return rc;
-    from.norm32 = norm32;
     return scale_launches(tensors, count, from, as_stream(stream));
 }
 
