@@ -290,41 +290,72 @@ py::object clip(const py::list& parameters, int kind, double limit, int device, 
     return py::reinterpret_steal<py::object>(THPVariable_Wrap(norm));
 }
 
-// fp32 values of 8-bit states (dicts that hold what a step left there), all on one device
-py::object moments(const py::list& states, uintptr_t stream) {
+// fp32 tensor of `like`'s sizes and strides in `flat`'s memory, without the dispatcher's round that as_strided() makes
+py::object part_of(const at::Tensor& flat, int64_t at, const at::Tensor& like) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(), flat.dtype());
+    impl->set_storage_offset(at);
+    impl->set_sizes_and_strides(like.sizes(), like.strides());
+    return py::reinterpret_steal<py::object>(THPVariable_Wrap(at::Tensor(std::move(impl))));
+}
+
+// the moments of all parameters in fp32: the state's own tensors where they are held in 32 bits, the codes' values where in 8
+// (of one device; OTHER_ORDER: of several), zeros where there is no state yet
+py::object moments(const py::list& param_groups, const py::dict& state, int device, uintptr_t stream) {
     const Keys& k = keys();
     std::vector<rfx_moment_tensor> rows;
-    std::vector<at::Tensor> like;
-    int64_t total = 0;
-    for (const auto& st : states) {
-        const at::Tensor &m = tensor(item(st.ptr(), k.exp_avg)), &v = tensor(item(st.ptr(), k.exp_avg_sq)), &e = tensor(item(st.ptr(), k.exponents));
-        if (m.scalar_type() != at::kByte || v.scalar_type() != at::kByte || e.scalar_type() != at::kChar || !m.is_cuda() || v.device() != m.device()
-            || e.device() != m.device() || m.sizes() != v.sizes() || m.strides() != v.strides() || !m.is_non_overlapping_and_dense() || !e.is_contiguous()
-            || e.numel() != 2 * ((m.numel() + RFX_ADAMW_BLOCK - 1) / RFX_ADAMW_BLOCK) || (!like.empty() && m.device() != like[0].device()))
-            throw py::value_error("this is not the state of 8-bit moments");
-        rfx_moment_tensor r{};
-        r.exp_avg = static_cast<const uint8_t*>(m.data_ptr());
-        r.exp_avg_sq = static_cast<const uint8_t*>(v.data_ptr());
-        r.exponents = static_cast<const int8_t*>(e.data_ptr());
-        r.n = m.numel();
-        total += (r.n + 3) & ~(int64_t)3;                                  // every output at a multiple of 16 bytes
-        rows.push_back(r);
-        like.push_back(m);
-    }
+    std::vector<std::pair<size_t, at::Tensor>> codes;
     py::list avg, avg_sq;
-    if (rows.empty()) return py::make_tuple(avg, avg_sq);
-    const at::Tensor flat = at::empty({2 * total}, at::TensorOptions().dtype(at::kFloat).device(like[0].device()));
-    float* base = static_cast<float*>(flat.data_ptr());
-    int64_t at = 0;
-    for (size_t i = 0; i < rows.size(); ++i) {
-        rows[i].out_avg = base + at;
-        rows[i].out_avg_sq = base + total + at;
-        avg.append(py::reinterpret_steal<py::object>(THPVariable_Wrap(flat.as_strided(like[i].sizes(), like[i].strides(), at))));
-        avg_sq.append(py::reinterpret_steal<py::object>(THPVariable_Wrap(flat.as_strided(like[i].sizes(), like[i].strides(), total + at))));
-        at += (rows[i].n + 3) & ~(int64_t)3;
+    int64_t total = 0;
+    for (const auto& g : param_groups) {
+        for (const auto& p : py::reinterpret_borrow<py::list>(item(g.ptr(), k.params))) {
+            PyObject* st = PyDict_GetItemWithError(state.ptr(), p.ptr());
+            if (!st && PyErr_Occurred()) throw py::error_already_set();
+            if (!st || PyDict_Size(st) == 0) {
+                const at::Tensor like = tensor(p.ptr()).detach();
+                for (py::list* to : {&avg, &avg_sq})
+                    to->append(py::reinterpret_steal<py::object>(THPVariable_Wrap(at::zeros_like(like, like.options().dtype(at::kFloat)))));
+                continue;
+            }
+            PyObject *om = item(st, k.exp_avg), *ov = item(st, k.exp_avg_sq);
+            const at::Tensor &m = tensor(om), &v = tensor(ov);
+            if (m.scalar_type() != at::kByte) {                            // (torch's own step on the CPU holds them in the parameter's type)
+                const bool as_is = m.scalar_type() == at::kFloat && v.scalar_type() == at::kFloat;
+                avg.append(as_is ? py::reinterpret_borrow<py::object>(om) : py::reinterpret_steal<py::object>(THPVariable_Wrap(m.to(at::kFloat))));
+                avg_sq.append(as_is ? py::reinterpret_borrow<py::object>(ov) : py::reinterpret_steal<py::object>(THPVariable_Wrap(v.to(at::kFloat))));
+                continue;
+            }
+            const at::Tensor& e = tensor(item(st, k.exponents));
+            if (v.scalar_type() != at::kByte || e.scalar_type() != at::kChar || !m.is_cuda() || v.device() != m.device() || e.device() != m.device()
+                || m.sizes() != v.sizes() || m.strides() != v.strides() || !m.is_non_overlapping_and_dense() || !e.is_contiguous()
+                || e.numel() != 2 * ((m.numel() + RFX_ADAMW_BLOCK - 1) / RFX_ADAMW_BLOCK))
+                throw py::value_error("this is not the state of 8-bit moments");
+            if (m.device().index() != device) return py::int_((int)OTHER_ORDER);
+            rfx_moment_tensor r{};
+            r.exp_avg = static_cast<const uint8_t*>(m.data_ptr());
+            r.exp_avg_sq = static_cast<const uint8_t*>(v.data_ptr());
+            r.exponents = static_cast<const int8_t*>(e.data_ptr());
+            r.n = m.numel();
+            total += (r.n + 3) & ~(int64_t)3;                              // every output at a multiple of 16 bytes
+            rows.push_back(r);
+            codes.emplace_back(avg.size(), m);
+            avg.append(py::none());
+            avg_sq.append(py::none());
+        }
     }
-    const int rc = rfx.adamw_moments(rows.data(), (int)rows.size(), (rfx_stream)stream);
-    if (rc != RFX_OK) return py::int_(rc);
+    if (!rows.empty()) {
+        const at::Tensor flat = at::empty({2 * total}, at::TensorOptions().dtype(at::kFloat).device(codes[0].second.device()));
+        float* base = static_cast<float*>(flat.data_ptr());
+        int64_t at = 0;
+        for (size_t i = 0; i < rows.size(); ++i) {
+            rows[i].out_avg = base + at;
+            rows[i].out_avg_sq = base + total + at;
+            avg[codes[i].first] = part_of(flat, at, codes[i].second);
+            avg_sq[codes[i].first] = part_of(flat, total + at, codes[i].second);
+            at += (rows[i].n + 3) & ~(int64_t)3;
+        }
+        const int rc = rfx.adamw_moments(rows.data(), (int)rows.size(), (rfx_stream)stream);
+        if (rc != RFX_OK) return py::int_(rc);
+    }
     return py::make_tuple(avg, avg_sq);
 }
 

@@ -589,28 +589,43 @@ static bool group_ok(const rfx_adamw_group& g) {
     return (g.state_bits == 32 || g.state_bits == 8) && g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0 && g.eps >= 0.0;
 }
 
-static bool overlap(const rfx_adamw_tensor& a, const rfx_adamw_tensor& b) {
-    const uintptr_t a0 = (uintptr_t)a.param, b0 = (uintptr_t)b.param;
-    return a0 < b0 + (uintptr_t)b.n * elem_bytes(b.dtype) && b0 < a0 + (uintptr_t)a.n * elem_bytes(a.dtype);
-}
+// memory that a launch writes: no two of its tensors may share any.  Tensors mostly lie one behind the other, outside of all before
+struct Written {
+    uintptr_t from[GN_TENSORS], to[GN_TENSORS], least = ~(uintptr_t)0, most = 0;
+    int count = 0;
+    void clear() { count = 0; least = ~(uintptr_t)0; most = 0; }
+    bool shares(const void* p, int64_t bytes) const {
+        const uintptr_t a = (uintptr_t)p, b = a + (uintptr_t)bytes;
+        if (a >= most || b <= least) return false;
+        for (int i = 0; i < count; ++i)
+            if (a < to[i] && from[i] < b) return true;
+        return false;
+    }
+    void add(const void* p, int64_t bytes) {
+        from[count] = (uintptr_t)p;
+        to[count] = from[count] + (uintptr_t)bytes;
+        least = from[count] < least ? from[count] : least;
+        most = to[count] > most ? to[count] : most;
+        ++count;
+    }
+};
+static_assert(AW_TENSORS <= GN_TENSORS, "");
 
 // pieces of the gradients [at, at + as many as fit) as one launch; returns how many were taken, 0: none left, < 0: an error.
 // apart: no two of a launch share memory (they are written)
 static int gather(const rfx_grad_tensor* t, int count, int& at, GnArgs& k, int piece, bool apart) {
     int64_t pieces = 0;
+    Written written;
     k.count = 0;
     k.piece = piece;
     for (; at < count && k.count < GN_TENSORS; ++at) {
         if (t[at].n == 0) continue;
-        bool shared = false;
-        for (int j = 0; apart && !shared && j < k.count; ++j) {
-            const uintptr_t a = (uintptr_t)t[at].grad, b = (uintptr_t)k.t[j].g;
-            shared = a < b + (uintptr_t)k.t[j].n * elem_bytes(k.dtype[j]) && b < a + (uintptr_t)t[at].n * elem_bytes(t[at].dtype);
-        }
-        if (shared) break;
+        const int64_t size = t[at].n * elem_bytes(t[at].dtype);
+        if (apart && written.shares(t[at].grad, size)) break;
         const int64_t p = (t[at].n + piece - 1) / piece;
         if (p > 0x7fffffff) return RFX_ERR_UNSUPPORTED;
         if (pieces + p > 0x7fffffff) break;
+        if (apart) written.add(t[at].grad, size);
         k.t[k.count].g = t[at].grad;
         k.t[k.count].n = t[at].n;
         k.dtype[k.count] = (uint8_t)t[at].dtype;
@@ -746,8 +761,9 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
         if (!(kinds >> kind & 1)) continue;
         for (int counted = 0; counted < 2; ++counted) {                    // step counts from the host, then those on the device
             if (counted && !on_device) break;
-            int at[AW_TENSORS], group_at[AW_GROUPS], used = 0;
+            int group_at[AW_GROUPS], used = 0;
             int64_t blocks = 0;
+            Written written;
             k.count = 0;
             k.dev = nullptr;
             for (int i = 0; i <= count; ++i) {
@@ -758,20 +774,20 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
                     const int64_t pieces = pieces_of(t.n);
                     int gi = 0;
                     while (gi < used && group_at[gi] != t.group) ++gi;
-                    bool full = k.count == AW_TENSORS || gi == AW_GROUPS || blocks + pieces > 0x7fffffff;
-                    for (int j = 0; !full && j < k.count; ++j) full = overlap(t, tensors[at[j]]);
-                    if (!full) {
+                    const int64_t size = t.n * elem_bytes(t.dtype);
+                    if (k.count < AW_TENSORS && gi < AW_GROUPS && blocks + pieces <= 0x7fffffff && !written.shares(t.param, size)) {
                         if (gi == used) {
                             const rfx_adamw_group& g = groups[t.group];
                             AwGroup& a = k.group[gi];
                             a.b1 = g.beta1; a.c1 = 1.0 - g.beta1; a.b2 = g.beta2; a.c2 = 1.0 - g.beta2;
                             a.eps = (float)g.eps;
+                            if (g.state_bits == 8 && g.eps > 0.0 && a.eps < 1.17549435e-38f) a.eps = 1.17549435e-38f;    // rcp takes less for 0
                             a.sign = g.maximize ? -1.f : 1.f;
                             if (!counted) a.s = step_scalars(g.lr, g.beta1, g.beta2, g.weight_decay, (double)g.step, g.seed);
                             prep.g[gi] = {g.lr, g.beta1, g.beta2, g.weight_decay, g.lr_dev, g.seed};
                             group_at[used++] = t.group;
                         }
-                        at[k.count] = i;
+                        written.add(t.param, size);
                         k.t[k.count] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exponents, t.master, t.n, gi, t.index};
                         prep.step[k.count] = t.step_dev;
                         prep.group[k.count] = (uint8_t)gi;
@@ -786,6 +802,7 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
                 if (rc != RFX_OK) return rc;
                 used = 0;
                 blocks = 0;
+                written.clear();
             }
         }
     }

@@ -181,8 +181,6 @@ def _check_grad(g):
         raise _lib.RfxError("sparse gradients are not supported")
     if g.dtype not in _lib.DTYPES:
         raise _lib.RfxError(f"gradients of type {g.dtype} are not supported: float32, bfloat16 or float16")
-    if _overlaps_itself(g):
-        raise _lib.RfxError("a gradient whose elements share memory (an expanded tensor) is not supported")
 
 
 def _grad_rows(grads):
@@ -218,6 +216,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     dev = grads[0].device
     for g in grads:
         _check_grad(g)
+        if _overlaps_itself(g):
+            raise _lib.RfxError("a gradient whose elements share memory (an expanded tensor) cannot be scaled in place")
         if g.device != dev:
             raise _lib.RfxError("gradients on different devices: clip them device by device")
     flat = [g if _dense(g) else g.contiguous() for g in grads]
@@ -317,8 +317,15 @@ class AdamW(torch.optim.AdamW):
     def load_state_dict(self, state_dict):
         """as torch's, but moments and master weights keep their own types (torch casts them to the parameter's); a dict of
         torch.optim.AdamW fits groups with 32-bit moments"""
+        held = ("exp_avg", "exp_avg_sq", "exponents", "master")
         seen, mine = [], [{k: g[k] for k in self._own} for g in self.param_groups]
-        hook = self.register_load_state_dict_pre_hook(lambda opt, d: seen.append(d))
+
+        def without_held(opt, d):                            # the last of the hooks: what it keeps from torch is put in below
+            seen.append(d)
+            return {**d, "state": {i: {k: v for k, v in st.items() if k not in held} if isinstance(st, dict) else st
+                                   for i, st in d["state"].items()}}
+
+        hook = self.register_load_state_dict_pre_hook(without_held)
         try:
             super().load_state_dict(state_dict)
         finally:
@@ -328,9 +335,7 @@ class AdamW(torch.optim.AdamW):
             for i, p in zip(saved["params"], g["params"]):
                 st = seen[0]["state"].get(i)
                 if st:
-                    for key in ("exp_avg", "exp_avg_sq", "exponents", "master"):
-                        if key in st:
-                            self.state[p][key] = st[key].to(device=p.device)
+                    self.state[p].update({k: st[k].to(device=p.device) for k in held if k in st})
                     if p.is_cuda:
                         self._check_state(p, g)
 
@@ -400,29 +405,18 @@ class AdamW(torch.optim.AdamW):
     def moments(self):
         """(exp_avg, exp_avg_sq) of all parameters, in their order, as fp32 tensors: the state's own tensors where moments are held
         in 32 bits, the values of the codes where in 8, zeros where there is no state yet"""
-        avg, avg_sq, eight = [], [], {}
-        for g in self.param_groups:
-            for p in g["params"]:
-                st = self.state.get(p)
-                if st and st["exp_avg"].dtype is torch.uint8:
-                    at, states = eight.setdefault(st["exp_avg"].get_device(), ([], []))
-                    at.append(len(avg))
-                    states.append(st)
-                    m = v = None
-                elif st:
-                    m, v = st["exp_avg"], st["exp_avg_sq"]
-                else:
-                    m, v = (torch.zeros_like(p, dtype=torch.float32, requires_grad=False) for _ in range(2))
-                avg.append(m)
-                avg_sq.append(v)
-        for index, (at, states) in eight.items():
+        codes = [st["exp_avg"] for st in self.state.values() if st and st["exp_avg"].dtype is torch.uint8]
+        if not codes:
+            index = stream = 0
+            out = _lib.host().moments(self.param_groups, self.state, index, stream)
+        else:
+            index = codes[0].get_device()
             with _on(index):
-                out = _lib.host().moments(states, _lib.stream_ptr(index))
-            if isinstance(out, int):
-                _lib.check(out, "rfx_adamw_moments")
-            for i, m, v in zip(at, *out):
-                avg[i], avg_sq[i] = m, v
-        return avg, avg_sq
+                out = _lib.host().moments(self.param_groups, self.state, index, _lib.stream_ptr(index))
+        if isinstance(out, int):
+            _lib.check(min(out, 0), "rfx_adamw_moments")
+            raise _lib.RfxError("8-bit moments on several devices: one optimizer per device reads its own")
+        return out
 
     # ---- the step ---------------------------------------------------------------------------------------------------------
     def _build(self, every):

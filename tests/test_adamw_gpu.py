@@ -388,6 +388,93 @@ def test_strides_gaps_and_ragged_gradients():
         assert torch.equal(wide[:, :3], wide0[:, :3]) and torch.equal(wide[:, 53:], wide0[:, 53:])
 
 
+@pytest.mark.parametrize("shift", [0, 1, 4])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_nothing_around_the_tensors_is_touched(dtype, bits, shift):
+    """parameters, gradients, moments, exponents and master copies inside larger buffers, at every kind of alignment: what lies before and
+    behind stays as it was, and the step is the one of tensors of their own"""
+    from remixfusion_amd.optim import AdamW
+    T, n = DTYPES[dtype], 5000 + 3
+    gen = torch.Generator(device="cuda").manual_seed(40)
+    rows = -(-n // 256)
+
+    def inside(t, at):
+        buf = torch.full((t.numel() + 2 * 64,), 77, dtype=t.dtype, device="cuda")
+        view = buf[at + 16:at + 16 + t.numel()].view(t.shape)
+        view.copy_(t)
+        return buf, view
+
+    init, grad = (torch.randn(n, device="cuda", generator=gen).to(T) for _ in range(2))
+    kind = torch.float32 if bits == 32 else torch.uint8
+    state = {"exp_avg": torch.zeros(n, device="cuda", dtype=kind), "exp_avg_sq": torch.zeros(n, device="cuda", dtype=kind)}
+    if bits == 8:
+        state["exponents"] = torch.full((2, rows), -127, device="cuda", dtype=torch.int8)
+    if dtype != "f32":
+        state["master"] = init.float()
+    around, out = [], []
+    for wrap in (False, True):
+        p, g, st = init.clone(), grad.clone(), {k: v.clone() for k, v in state.items()}
+        if wrap:
+            bufs = {}
+            bufs["p"], p = inside(p, shift)
+            bufs["g"], g = inside(g, shift)
+            for k in list(st):
+                bufs[k], st[k] = inside(st[k], 4 * shift if bits == 8 and k in ("exp_avg", "exp_avg_sq") else shift)
+        p = torch.nn.Parameter(p)
+        p.grad = g
+        opt = AdamW([p], lr=0.01, state_bits=bits, master_weights=dtype != "f32", seed=3)
+        opt.load_state_dict({"state": {0: {"step": torch.tensor(0.0), **st}}, "param_groups": opt.state_dict()["param_groups"]})
+        for _ in range(3):
+            opt.step()
+        if wrap:
+            for k, v in st.items():
+                assert opt.state[p][k].data_ptr() == v.data_ptr(), k               # stepped where it lies
+            for k, buf in bufs.items():
+                at = (4 * shift if bits == 8 and k in ("exp_avg", "exp_avg_sq") else shift) + 16
+                size = {"exponents": 2 * rows}.get(k, n)
+                assert bool((buf[:at] == 77).all()) and bool((buf[at + size:] == 77).all()), k
+        out.append([p.detach().clone()] + [opt.state[p][k].clone() for k in st])
+    for a, b in zip(*out):
+        assert torch.equal(a.reshape(-1), b.reshape(-1))
+
+
+def test_states_at_odd_addresses():
+    """8-bit moments that were loaded from an address no word starts at are brought to one; an expanded gradient is read as what it stands for"""
+    from remixfusion_amd.optim import AdamW
+    p, q = (torch.nn.Parameter(torch.ones(700, device="cuda")) for _ in range(2))
+    buf = torch.zeros(1500, dtype=torch.uint8, device="cuda")
+    a, b = (AdamW([x], lr=0.1, state_bits=8) for x in (p, q))
+    a.load_state_dict({"state": {0: {"step": torch.tensor(0.0), "exp_avg": buf[1:701], "exp_avg_sq": buf[703:1403],
+                                     "exponents": torch.full((2, 3), -127, dtype=torch.int8, device="cuda")}},
+                       "param_groups": a.state_dict()["param_groups"]})
+    p.grad = torch.full((1,), 0.25, device="cuda").expand(700)
+    q.grad = torch.full((700,), 0.25, device="cuda")
+    a.step(); b.step()
+    assert torch.equal(p, q) and torch.equal(a.state[p]["exp_avg"], b.state[q]["exp_avg"]) and int(buf.max()) == 0
+    from remixfusion_amd import _lib as L
+    from remixfusion_amd.optim import clip_grad_norm_
+    with pytest.raises(L.RfxError):
+        clip_grad_norm_([p], 1.0)                                                  # which cannot be written
+
+
+def test_learning_rates_on_the_device():
+    from remixfusion_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    p.grad = torch.ones_like(p)
+    for lr in (torch.tensor(0.1), torch.tensor([0.1, 0.1], device="cuda"), torch.tensor(0.1, device="cuda", dtype=torch.float64)):
+        with pytest.raises(ValueError):
+            AdamW([p], lr=lr, capturable=True).step()
+    assert float(p.detach().min()) == 1.0
+    AdamW([p], lr=torch.tensor([0.1], device="cuda"), capturable=True, weight_decay=0.0).step()
+    assert abs(float(p.detach()[0]) - 0.9) < 1e-6
+    # eps below fp32's normal numbers, no gradient: nothing happens
+    z = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    z.grad = torch.zeros_like(z)
+    AdamW([z], state_bits=8, eps=1e-42, weight_decay=0.0).step()
+    assert bool((z == 1).all())
+
+
 def test_parameters_that_share_memory_step_one_after_the_other():
     from remixfusion_amd.optim import AdamW
     gen = torch.Generator(device="cuda").manual_seed(4)
