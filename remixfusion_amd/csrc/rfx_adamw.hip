@@ -504,15 +504,7 @@ template <typename T> __device__ __forceinline__ void scale_piece(T* g, int len,
     int done = 0;
     if (((uintptr_t)g & (4 * sizeof(T) - 1)) == 0) {
         done = len & ~3;
-        int i = threadIdx.x * 4;
-        for (; i + 3 * SC_THREADS * 4 < done; i += 4 * SC_THREADS * 4) {
-            const f4 x = load4(g + i), y = load4(g + i + SC_THREADS * 4), z = load4(g + i + 2 * SC_THREADS * 4), w = load4(g + i + 3 * SC_THREADS * 4);
-            store4(g + i, x * c);
-            store4(g + i + SC_THREADS * 4, y * c);
-            store4(g + i + 2 * SC_THREADS * 4, z * c);
-            store4(g + i + 3 * SC_THREADS * 4, w * c);
-        }
-        for (; i < done; i += SC_THREADS * 4) store4(g + i, load4(g + i) * c);
+        for (int i = threadIdx.x * 4; i < done; i += SC_THREADS * 4) store4(g + i, load4(g + i) * c);
     }
     for (int i = done + threadIdx.x; i < len; i += SC_THREADS) g[i] = (T)((float)g[i] * c);
 }
@@ -635,9 +627,9 @@ static int gather(const rfx_grad_tensor* t, int count, int& at, GnArgs& k, int m
         all += t[at].n;
     }
     const auto whole = [](int64_t n) { const int64_t r = n > 4 * GN_ROUND ? 4 * GN_ROUND : GN_ROUND; return (n + r - 1) / r * r; };
-    const auto pieces_at = [&](int64_t piece) {                            // a remainder under an eighth is not worth a longer piece for all
+    const auto pieces_at = [&](int64_t piece) {
         int64_t n = 0;
-        for (int i = 0; i < k.count; ++i) n += (k.t[i].n + piece - 1 - piece / 8) / piece;
+        for (int i = 0; i < k.count; ++i) n += (k.t[i].n + piece - 1) / piece;
         return n;
     };
     int64_t piece = whole(all / most + 1);
