@@ -45,8 +45,8 @@ struct AwGroup {
     float sign;                         // -1: maximize
 };
 
-// Where the clipping factor comes from: partial sums (maxima) of the norm that every block joins for itself -- at most as many as a
-// block has threads, so this is one load a thread out of L2 and a launch less -- or a factor that is there.  Neither: no clipping.
+// Where the clipping factor comes from: partial sums (maxima) of the norm that every wave joins for itself -- never more than four a
+// lane, out of L2, for a launch less -- or a factor that is there.  Neither: no clipping.
 constexpr int JOIN = 256;
 struct ClipSource {
     const double* partial;
@@ -155,11 +155,21 @@ __device__ __forceinline__ double factor_of(double norm, double max_norm) {
     return f > 1.0 ? 1.0 : f;                                              // NaN stays NaN
 }
 
-// for blocks of JOIN threads
+// each wave for itself, so that nothing waits at a barrier
 __device__ __forceinline__ double clip_factor(const ClipSource& c) {
     if (c.n == 0) return c.factor ? c.factor[1] : 1.0;
-    __shared__ double lds[JOIN / 64];
-    const double x = block_join<JOIN>((int)threadIdx.x < c.n ? c.partial[threadIdx.x] : 0.0, c.max != 0, lds);
+    double x = 0.0;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < JOIN; i += 64) {
+        const double y = i + lane < c.n ? c.partial[i + lane] : 0.0;
+        x = c.max ? larger(x, y) : x + y;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        const double y = __shfl_xor(x, d, 64);
+        x = c.max ? larger(x, y) : x + y;
+    }
     const double norm = c.max ? x : sqrt(x);
     if (c.norm32 && blockIdx.x == 0 && threadIdx.x == 0) *c.norm32 = (float)norm;
     return factor_of(norm, c.max_norm);
@@ -498,18 +508,18 @@ __global__ __launch_bounds__(JOIN) void grad_norm_join_kernel(const double* part
     if (norm32) *norm32 = (float)norm;
 }
 
-constexpr int SC_THREADS = JOIN;
-constexpr int SC_BLOCKS = 2048;         // eight a CU: what is resident at once
+// the norm's pieces on the blocks that the norm had them on: what an XCD's L2 still holds of a small set is found there (1.6 million
+// gradients 5.0 us, in pieces of another size 7.4)
 template <typename T> __device__ __forceinline__ void scale_piece(T* g, int len, float c) {
     int done = 0;
     if (((uintptr_t)g & (4 * sizeof(T) - 1)) == 0) {
         done = len & ~3;
-        for (int i = threadIdx.x * 4; i < done; i += SC_THREADS * 4) store4(g + i, load4(g + i) * c);
+        for (int i = threadIdx.x * 4; i < done; i += GN_THREADS * 4) store4(g + i, load4(g + i) * c);
     }
-    for (int i = done + threadIdx.x; i < len; i += SC_THREADS) g[i] = (T)((float)g[i] * c);
+    for (int i = done + threadIdx.x; i < len; i += GN_THREADS) g[i] = (T)((float)g[i] * c);
 }
 
-__global__ __launch_bounds__(SC_THREADS) void grad_scale_kernel(const GnArgs k) {
+__global__ __launch_bounds__(GN_THREADS) void grad_scale_kernel(const GnArgs k) {
     const double f = clip_factor(k.clip);
     if (f == 1.0) return;
     const float c = (float)f;
@@ -627,9 +637,9 @@ static int gather(const rfx_grad_tensor* t, int count, int& at, GnArgs& k, int m
         all += t[at].n;
     }
     const auto whole = [](int64_t n) { const int64_t r = n > 4 * GN_ROUND ? 4 * GN_ROUND : GN_ROUND; return (n + r - 1) / r * r; };
-    const auto pieces_at = [&](int64_t piece) {
+    const auto pieces_at = [&](int64_t piece) {                            // a remainder under an eighth is not worth a longer piece for all
         int64_t n = 0;
-        for (int i = 0; i < k.count; ++i) n += (k.t[i].n + piece - 1) / piece;
+        for (int i = 0; i < k.count; ++i) n += (k.t[i].n + piece - 1 - piece / 8) / piece;
         return n;
     };
     int64_t piece = whole(all / most + 1);
@@ -654,10 +664,10 @@ static bool grads_ok(const rfx_grad_tensor* t, int count) {
     return true;
 }
 
-// Blocks of the 8-bit step from which the partial results are joined in a launch of their own.  A clipped step, us (every block / a launch):
-// 0.1 million parameters 9.2 / 11.5, 4 million 23.7 / 23.4, 16 million 70 / 65, 40 million 159 / 143.  The 32-bit step waits for memory
-// anyway: 11.7 / 12.9, 28.0 / 28.6, 90.1 / 90.6, 197.4 / 198.0.
-constexpr int64_t JOIN_BLOCKS = 4096;
+// Blocks of a step from which the partial results are joined in a launch of their own.  A clipped step, us (every wave / a launch), 32 bits:
+// 0.1 million parameters 11.3 / 13.5, 2 million 17.4 / 17.6, 8 million 46.6 / 45.7, 40 million 194.7 / 192.8; 8 bits: 11.2 / 11.8,
+// 16.6 / 16.7, 38.0 / 34.6, 158 / 139.
+constexpr int64_t JOIN_BLOCKS = 2048;
 
 static size_t partials(int count) { return (size_t)JOIN * ((count + GN_TENSORS - 1) / GN_TENSORS) + 2; }
 
@@ -698,9 +708,9 @@ static int no_norm(const double* workspace, float* norm32, hipStream_t stream) {
 
 static int scale_launches(const rfx_grad_tensor* tensors, int count, ClipSource from, hipStream_t stream) {
     GnArgs k;
-    for (int at = 0; gather(tensors, count, at, k, SC_BLOCKS, true) > 0;) {
+    for (int at = 0; gather(tensors, count, at, k, JOIN, true) > 0;) {
         k.clip = from;
-        hipLaunchKernelGGL(grad_scale_kernel, dim3(k.pieces < SC_BLOCKS ? k.pieces : SC_BLOCKS), dim3(SC_THREADS), 0, stream, k);
+        hipLaunchKernelGGL(grad_scale_kernel, dim3(k.pieces < JOIN ? k.pieces : JOIN), dim3(GN_THREADS), 0, stream, k);
         RFX_LAUNCH_CHECK();
         from.norm32 = nullptr;
     }
@@ -725,7 +735,7 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
     if (!tensors || count < 0 || !groups || n_groups < 1) return RFX_ERR_ARG;
     bool on_device = false;
     unsigned kinds = 0;
-    int64_t bytes = 0, blocks8 = 0;
+    int64_t bytes = 0, blocks_in_all = 0;
     for (int i = 0; i < n_groups; ++i)
         if (!group_ok(groups[i])) return RFX_ERR_ARG;
     for (int i = 0; i < count; ++i) {
@@ -734,7 +744,7 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
         on_device |= tensors[i].step_dev != nullptr;
         kinds |= 1U << kind_of(tensors[i], groups[tensors[i].group]);
         bytes += tensors[i].n * (2 * elem_bytes(tensors[i].dtype) + (tensors[i].master ? 4 : 0) + (groups[tensors[i].group].state_bits == 8 ? 2 : 8));
-        if (groups[tensors[i].group].state_bits == 8) blocks8 += pieces_of(tensors[i].n);
+        blocks_in_all += pieces_of(tensors[i].n);
     }
     if (clip_grads && (!grads_ok(clip_grads, count) || !(max_norm >= 0.0))) return RFX_ERR_ARG;
     if ((on_device || clip_grads) && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < rfx_adamw_workspace_bytes(count)))
@@ -748,7 +758,7 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
         int n = 0;
         double* at = (double*)((char*)workspace + (size_t)count * sizeof(AwStep));
         int rc = norm_launches(clip_grads, count, 0, max_norm, at, n, k.clip, as_stream(stream));
-        if (rc == RFX_OK) rc = join(at, n, blocks8, norm32, k.clip, as_stream(stream));
+        if (rc == RFX_OK) rc = join(at, n, blocks_in_all, norm32, k.clip, as_stream(stream));
         if (rc != RFX_OK) return rc;
     }
     for (int kind = 0; kind < 12; ++kind) {
