@@ -67,6 +67,11 @@ struct Keys {
 };
 const Keys& keys() { static const Keys* k = new Keys; return *k; }
 
+// autograd notices a tensor that is written behind its back only by its version
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // what a step's outcome is to the caller: a negative status of librfx, or one of these
 enum Outcome { DONE = 0, STALE = 1, OTHER_ORDER = 2 };
 
@@ -257,8 +262,10 @@ private:
         const int rc = rfx.adamw_step(rows.data(), (int)n, groups_.data(), (int)groups_.size(), limit >= 0.0 ? grads_.data() : nullptr, limit, norm32,
                                       bytes ? ws.data_ptr() : nullptr, bytes, (rfx_stream)stream);
         if (rc != RFX_OK) return py::int_(rc);
-        for (size_t i = 0; i < n; ++i)
+        for (size_t i = 0; i < n; ++i) {
             if (counts_[i]) *counts_[i] += 1.f;
+            written(tensor(params_[i].ptr()));
+        }
         return norm;
     }
 };
@@ -287,6 +294,10 @@ py::object clip(const py::list& parameters, int kind, double limit, int device, 
     const int rc = rfx.grad_clip(rows.data(), (int)rows.size(), kind, limit, static_cast<float*>(norm.data_ptr()), ws.data_ptr(), bytes,
                                  (rfx_stream)stream);
     if (rc != RFX_OK) return py::int_(rc);
+    for (const auto& o : parameters) {
+        const at::Tensor& g = tensor(o.ptr()).grad();
+        if (g.defined()) written(g);
+    }
     return py::reinterpret_steal<py::object>(THPVariable_Wrap(norm));
 }
 

@@ -541,6 +541,8 @@ static int elem_bytes(int dtype) { return dtype == RFX_F32 ? 4 : 2; }
 // 128 MB 46 / 43, 665 MB 222 / 204; behind other work on 256 MB, as in a training loop, 16 MB 13.8 / 8.1, 64 MB 44 / 26, 128 MB 68 / 44.
 constexpr int64_t STREAM_BYTES = 64 << 20;
 static int64_t pieces_of(int64_t n) { return (n + AW_PIECE - 1) / AW_PIECE; }
+constexpr int64_t AW_BLOCKS = 0xffffffffLL / AW_THREADS;                   // of a launch: its threads are counted in 32 bits
+constexpr int64_t MOST_ELEMENTS = (int64_t)1 << 52;                        // sizes add up without overflow
 
 // one launch of the tensors gathered in `k`; dev: their scalars' place in the workspace (step counts on the device)
 static int adamw_launch(AwArgs& k, PrepArgs* prep, int kind, bool past, hipStream_t stream) {
@@ -582,7 +584,7 @@ static int adamw_launch(AwArgs& k, PrepArgs* prep, int kind, bool past, hipStrea
 static int kind_of(const rfx_adamw_tensor& t, const rfx_adamw_group& g) { return t.dtype + (t.master ? 3 : 0) + (g.state_bits == 8 ? 6 : 0); }
 
 static bool tensor_ok(const rfx_adamw_tensor& t, const rfx_adamw_group* groups, int n_groups) {
-    if (t.n < 0 || t.group < 0 || t.group >= n_groups || t.dtype < RFX_F32 || t.dtype > RFX_F16) return false;
+    if (t.n < 0 || t.n > MOST_ELEMENTS || t.group < 0 || t.group >= n_groups || t.dtype < RFX_F32 || t.dtype > RFX_F16) return false;
     const rfx_adamw_group& g = groups[t.group];
     if (!t.step_dev && (g.step < 1 || g.lr_dev)) return false;
     if (t.master && t.dtype == RFX_F32) return false;
@@ -657,8 +659,7 @@ static int gather(const rfx_grad_tensor* t, int count, int& at, GnArgs& k, int m
 static bool grads_ok(const rfx_grad_tensor* t, int count) {
     if (count < 0 || (count > 0 && !t)) return false;
     for (int i = 0; i < count; ++i) {
-        if (t[i].n < 0 || t[i].dtype < RFX_F32 || t[i].dtype > RFX_F16) return false;
-        if (t[i].n > (int64_t)1 << 52) return false;                       // sizes add up without overflow
+        if (t[i].n < 0 || t[i].n > MOST_ELEMENTS || t[i].dtype < RFX_F32 || t[i].dtype > RFX_F16) return false;
         if (t[i].n > 0 && (!t[i].grad || ((uintptr_t)t[i].grad & (uintptr_t)(elem_bytes(t[i].dtype) - 1)))) return false;
     }
     return true;
@@ -740,7 +741,7 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
         if (!group_ok(groups[i])) return RFX_ERR_ARG;
     for (int i = 0; i < count; ++i) {
         if (!tensor_ok(tensors[i], groups, n_groups)) return RFX_ERR_ARG;
-        if (pieces_of(tensors[i].n) > 0x7fffffff) return RFX_ERR_UNSUPPORTED;
+        if (pieces_of(tensors[i].n) > AW_BLOCKS) return RFX_ERR_UNSUPPORTED;
         on_device |= tensors[i].step_dev != nullptr;
         kinds |= 1U << kind_of(tensors[i], groups[tensors[i].group]);
         bytes += tensors[i].n * (2 * elem_bytes(tensors[i].dtype) + (tensors[i].master ? 4 : 0) + (groups[tensors[i].group].state_bits == 8 ? 2 : 8));
@@ -779,7 +780,7 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
                     int gi = 0;
                     while (gi < used && group_at[gi] != t.group) ++gi;
                     const int64_t size = t.n * elem_bytes(t.dtype);
-                    if (k.count < AW_TENSORS && gi < AW_GROUPS && blocks + pieces <= 0x7fffffff && !written.shares(t.param, size)) {
+                    if (k.count < AW_TENSORS && gi < AW_GROUPS && blocks + pieces <= AW_BLOCKS && !written.shares(t.param, size)) {
                         if (gi == used) {
                             const rfx_adamw_group& g = groups[t.group];
                             AwGroup& a = k.group[gi];
@@ -819,9 +820,9 @@ int rfx_adamw_moments(const rfx_moment_tensor* tensors, int count, rfx_stream st
     int64_t bytes = 0;
     for (int i = 0; i < count; ++i) {
         const rfx_moment_tensor& t = tensors[i];
-        if (t.n < 0 || (t.n > 0 && (!t.exp_avg || !t.exp_avg_sq || !t.exponents || !t.out_avg || !t.out_avg_sq))) return RFX_ERR_ARG;
+        if (t.n < 0 || t.n > MOST_ELEMENTS || (t.n > 0 && (!t.exp_avg || !t.exp_avg_sq || !t.exponents || !t.out_avg || !t.out_avg_sq))) return RFX_ERR_ARG;
         if (((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq | (uintptr_t)t.out_avg | (uintptr_t)t.out_avg_sq) & 3) return RFX_ERR_ARG;
-        if (pieces_of(t.n) > 0x7fffffff) return RFX_ERR_UNSUPPORTED;
+        if (pieces_of(t.n) > AW_BLOCKS) return RFX_ERR_UNSUPPORTED;
         bytes += 8 * t.n;                                                  // of the outputs: 332 MB of them 72 us plain, 61 past the caches
     }
     MomArgs k;
@@ -830,7 +831,7 @@ int rfx_adamw_moments(const rfx_moment_tensor* tensors, int count, rfx_stream st
         for (k.count = 0; i < count && k.count < AW_TENSORS; ++i) {
             if (tensors[i].n == 0) continue;
             const int64_t pieces = pieces_of(tensors[i].n);
-            if (blocks + pieces > 0x7fffffff) break;
+            if (blocks + pieces > AW_BLOCKS) break;
             k.t[k.count] = tensors[i];
             k.first[k.count++] = (int32_t)blocks;
             blocks += pieces;

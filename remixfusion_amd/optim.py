@@ -336,6 +336,8 @@ class AdamW(torch.optim.AdamW):
                 st = seen[0]["state"].get(i)
                 if st:
                     self.state[p].update({k: st[k].to(device=p.device) for k in held if k in st})
+                    if isinstance(self.state[p].get("step"), torch.Tensor):
+                        self.state[p]["step"] = self.state[p]["step"].detach().clone()      # (raised in place: not in the dict that was given)
                     if p.is_cuda:
                         self._check_state(p, g)
 
@@ -406,13 +408,11 @@ class AdamW(torch.optim.AdamW):
         """(exp_avg, exp_avg_sq) of all parameters, in their order, as fp32 tensors: the state's own tensors where moments are held
         in 32 bits, the values of the codes where in 8, zeros where there is no state yet"""
         codes = [st["exp_avg"] for st in self.state.values() if st and st["exp_avg"].dtype is torch.uint8]
-        if not codes:
-            index = stream = 0
-            out = _lib.host().moments(self.param_groups, self.state, index, stream)
-        else:
-            index = codes[0].get_device()
-            with _on(index):
-                out = _lib.host().moments(self.param_groups, self.state, index, _lib.stream_ptr(index))
+        if not codes:                                            # nothing to launch
+            return _lib.host().moments(self.param_groups, self.state, -1, 0)
+        index = codes[0].get_device()
+        with _on(index):
+            out = _lib.host().moments(self.param_groups, self.state, index, _lib.stream_ptr(index))
         if isinstance(out, int):
             _lib.check(min(out, 0), "rfx_adamw_moments")
             raise _lib.RfxError("8-bit moments on several devices: one optimizer per device reads its own")
@@ -422,7 +422,7 @@ class AdamW(torch.optim.AdamW):
     def _build(self, every):
         """plans for (parameter, its place in the optimizer, its group): states made or checked, one plan per device"""
         capturing = torch.cuda.is_current_stream_capturing()
-        by_device = {}
+        by_device, counts = {}, set()
         for entry in every:
             p, _, gi = entry
             g = self.param_groups[gi]
@@ -439,6 +439,10 @@ class AdamW(torch.optim.AdamW):
                 raise _lib.RfxError("the state is created by the first step() or prepare(): call it before capturing")
             else:
                 self._new_state(p, g)
+            st = self.state[p]
+            if st["step"].data_ptr() in counts:                  # one count for several parameters: each raises its own
+                st["step"] = st["step"].clone()
+            counts.add(st["step"].data_ptr())
         self._plans = {dev: (_lib.host().Plan(part, self.param_groups, self.state), part) for dev, part in by_device.items()}
 
     def step(self, closure=None):

@@ -139,7 +139,8 @@ def test_adamw_step_refusals_and_empty_calls():
     assert _call(None, None, 0, 0) == 0 and _call(None, _group()) == -1 and _call(_tensor(), None) == -1
     assert _call(_tensor(), _group(), -1) == -1 and _call(_tensor(), _group(), 1, 0) == -1
     assert _call(_tensor(n=0, param=None), _group()) == 0                               # no elements: nothing to launch
-    assert _call(_tensor(n=1 << 52), _group()) == -3
+    assert _call(_tensor(n=1 << 52), _group()) == -3 and _call(_tensor(n=(1 << 63) - 1), _group()) == -1
+    assert _call(_tensor(n=(1 << 34) + (1 << 20)), _group()) == -3                     # more blocks than a launch counts threads for
     lib = L.load()
     assert lib.rfx_adamw_workspace_bytes(0) == 0 and lib.rfx_adamw_workspace_bytes(-3) == 0 and lib.rfx_adamw_workspace_bytes(3) >= 48
     grads = (L.GradTensor * 1)(L.GradTensor(A + 4096, 8, 0, 0))

@@ -218,6 +218,87 @@ def test_many_tensors_equal_one_by_one(bits):
             assert torch.equal(one.state[q][key], opt.state[ps[i]][key])
 
 
+@pytest.mark.parametrize("bits,dtype,master", [(32, "f32", False), (8, "f32", False), (32, "bf16", True), (8, "f16", False), (8, "bf16", True)])
+def test_large_sets(bits, dtype, master):
+    """sizes whose loads and stores go past the caches, clipped by a norm that is joined in a launch of its own"""
+    from remixfusion_amd.optim import AdamW
+    T = DTYPES[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(19)
+    sizes = [11_000_003, 257, 40]                                                  # >= 64 MB in each of these forms
+    ps = [torch.nn.Parameter(torch.randn(n, device="cuda", generator=gen).mul(0.3).to(T)) for n in sizes]
+    opt = AdamW(ps, **SETTINGS[1], state_bits=bits, master_weights=master, seed=5, max_grad_norm=3.0)
+    refs = [Ref(p.detach().float().cpu().numpy(), bits, i, 5) for i, p in enumerate(ps)]
+    for it in range(2):
+        for p in ps:
+            p.grad = magnitudes(p.numel(), gen).to(T)
+        opt.step()
+        grads = [p.grad.double() for p in ps]
+        norm = math.sqrt(sum(float((g * g).sum()) for g in grads))
+        assert abs(float(opt.grad_norm) - norm) <= (U + 1e-12) * norm and norm > 3.0
+        for p, g, ref in zip(ps, grads, refs):
+            tp, tm, tv = ref.step(g.cpu().numpy(), **SETTINGS[1], c=3.0 / (norm + 1e-6), half=U if master else half_eps(T))
+            st = opt.state[p]
+            if bits == 8:
+                _check_code(st, ref, it)
+            else:
+                near(st["exp_avg"], ref.m, tm, "m"); near(st["exp_avg_sq"], ref.v, 2 * tv, "v")
+                ref.m, ref.v = (st[k].double().cpu().numpy() for k in ("exp_avg", "exp_avg_sq"))
+            near(st["master"] if master else p, ref.p, tp, "p")
+            ref.p = (st["master"] if master else p.detach()).double().cpu().numpy()
+    for p, ref, a, b in zip(ps, refs, *opt.moments()):
+        near(a, ref.m, 0.0, "moments"); near(b, ref.v, U * np.abs(ref.v) + 2.0 ** -149, "moments")
+
+
+def test_many_tensors_clipped():
+    """more partial results than a wave joins by itself: the step and clip_grad_norm_ against the formula"""
+    from remixfusion_amd.optim import AdamW, clip_grad_norm_
+    gen = torch.Generator(device="cuda").manual_seed(29)
+    ps = [torch.nn.Parameter(torch.randn(5000 + i, device="cuda", generator=gen)) for i in range(300)]
+    for p in ps:
+        p.grad = torch.randn(p.shape, device="cuda", generator=gen)
+    old, before = [p.grad.clone() for p in ps], [p.detach().clone() for p in ps]
+    norm = math.sqrt(sum(float((g.double() ** 2).sum()) for g in old))
+    opt = AdamW(ps, lr=0.1, betas=(0.5, 0.9), eps=1.0, weight_decay=0.0, max_grad_norm=10.0)
+    opt.step()
+    assert abs(float(opt.grad_norm) - norm) <= (U + 1e-12) * norm
+    c = 10.0 / (norm + 1e-6)
+    for p, g, x in zip(ps, old, before):                       # first step: m / (1 - b1) = c g, sqrt(v / (1 - b2)) = |c g|
+        want = x.double() - 0.1 * c * g.double() / (c * g.double().abs() + 1.0)
+        assert float((p.detach().double() - want).abs().max()) <= 4 * U * 8
+    for kind in (2.0, math.inf):
+        for p, g in zip(ps, old):
+            p.grad = g.clone()
+        n = clip_grad_norm_(ps, 1.0, kind)
+        want = norm if kind == 2.0 else max(float(g.abs().max()) for g in old)
+        assert abs(float(n) - want) <= (U + 1e-12) * want
+        for p, g in zip(ps, old):
+            assert float((p.grad.double() - g.double() / (want + 1e-6)).abs().max()) <= 3 * U * 8
+
+
+def test_what_autograd_and_others_notice():
+    """a step and a clipping raise the versions of what they write; a count that two parameters share is not raised twice"""
+    from remixfusion_amd.optim import AdamW, clip_grad_norm_
+    p, q = (torch.nn.Parameter(torch.ones(5, device="cuda")) for _ in range(2))
+    opt = AdamW([p, q], lr=0.1, capturable=True)
+    y = (p * p * q).sum()
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    v = p.grad._version
+    clip_grad_norm_([p], 0.5)
+    assert p.grad._version > v
+    opt.step()
+    with pytest.raises(RuntimeError):
+        y.backward()                                           # its saved p is not what it was
+    step = torch.tensor(3.0)
+    for cap in (False, True):
+        o = AdamW([p, q], lr=0.1, capturable=cap)
+        st = {"exp_avg": torch.zeros(5, device="cuda"), "exp_avg_sq": torch.zeros(5, device="cuda")}
+        o.load_state_dict({"state": {i: {"step": step, **{k: t.clone() for k, t in st.items()}} for i in range(2)},
+                           "param_groups": o.state_dict()["param_groups"]})
+        p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+        o.step(); o.step()
+        assert [float(o.state[x]["step"]) for x in (p, q)] == [5.0, 5.0]
+
+
 def test_against_torchs_adamw():
     """the fp32 step is torch.optim.AdamW's, and its state is read by torch and from torch"""
     from remixfusion_amd.optim import AdamW
@@ -781,6 +862,42 @@ def test_captured_steps_replay_like_eager_ones(bits):
     for p, q in zip(plain, fresh):
         assert float((p - q).detach().abs().max()) <= 4 * half_eps(p.dtype) * 4
         assert torch.equal(a.state[p]["exp_avg"], b.state[q]["exp_avg"])
+
+
+def test_clipping_and_reading_back_in_a_graph():
+    """clip_grad_norm_, step and moments() as one captured run, replayed on new gradients, against the same calls outside"""
+    from remixfusion_amd.optim import AdamW, clip_grad_norm_
+    gen = torch.Generator(device="cuda").manual_seed(37)
+    sizes = [3, 1000, 20001]
+    init = [torch.randn(n, device="cuda", generator=gen) for n in sizes]
+
+    def make():
+        ps = [torch.nn.Parameter(t.clone()) for t in init]
+        for p in ps:
+            p.grad = torch.zeros_like(p)
+        opt = AdamW(ps, lr=0.01, state_bits=8, capturable=True, seed=1)
+        opt.prepare()
+        return ps, opt
+
+    def run(ps, opt):
+        norm = clip_grad_norm_(ps, 0.5), clip_grad_norm_(ps, 1e9, math.inf)
+        opt.step()
+        return norm + tuple(opt.moments())
+
+    (ps, opt), (qs, ref) = make(), make()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        held = run(ps, opt)
+    for it in range(5):
+        for p, q in zip(ps, qs):
+            x = torch.randn(p.shape, device="cuda", generator=gen) * 10.0 ** (it - 3)         # over the limit, and under it
+            p.grad.copy_(x); q.grad.copy_(x)
+        g.replay()
+        torch.ones(1 << 20, device="cuda").sum().item()
+        out = run(qs, ref)
+        assert torch.equal(held[0], out[0]) and torch.equal(held[1], out[1]), it
+        for p, q, a, b, c, d in zip(ps, qs, held[2], out[2], held[3], out[3]):
+            assert torch.equal(p, q) and torch.equal(p.grad, q.grad) and torch.equal(a, b) and torch.equal(c, d), it
 
 
 def test_capture_needs_the_state_beforehand():

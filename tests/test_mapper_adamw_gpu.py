@@ -86,6 +86,14 @@ def test_one_map_iteration_is_the_formula(kind):
             i += 1
 
 
+def test_the_autograd_formulation_runs_with_it():
+    pipe = _pipeline(optimizer="adamw8bit", grad_clip=0.5, direct_iterations=False)
+    _run(pipe)
+    assert int(pipe.slam.mapping_idx[0]) == 10 and pipe.mapper._direct_iterations() is None
+    assert float(pipe.slam.map_optimizer.state[pipe.model.embed_res_fn.params]["step"]) == 5 + 2 * 5
+    assert all(bool(torch.isfinite(p).all()) for p in pipe.model.parameters() if p.requires_grad)
+
+
 def test_what_the_configuration_refuses():
     with pytest.raises(ValueError):
         _pipeline(optimizer="sgd")
