@@ -117,11 +117,10 @@ __host__ __device__ inline AwStep step_scalars(double lr, double b1, double b2, 
     return s;
 }
 
-// p - (lr wd p + step_size m / (sqrt(v) / sqrt(1 - b2^k) + eps)): the two small terms meet before they meet p, so a decay of less
-// than half a unit of p's last place is not lost to a rounding of its own
-__device__ __forceinline__ float stepped(float p, float m, float v, const AwStep& s, float eps) {
-    const float d = madd(sqrtf(v), s.inv_bc2, eps);
-    return p - madd(s.lr_wd, p, s.step_size * (m / d));
+// p - (lr wd p + update): the two small terms meet before they meet p, so a decay of less than half a unit of p's last place is not
+// lost to a rounding of its own.  An infinite p stays what p (1 - lr wd) leaves it
+__device__ __forceinline__ float stepped(float p, float update, float lr_wd) {
+    return p - (fabsf(p) == __builtin_inff() ? update : madd(lr_wd, p, update));
 }
 
 // ---- 32-bit moments: fp32 throughout ------------------------------------------------------------------------------------------
@@ -130,7 +129,7 @@ __device__ __forceinline__ void adamw_one(float& p, float g, float& m, float& v,
     g *= c;
     m = madd(c1, g, b1 * m);
     v = madd(c2 * g, g, b2 * v);
-    p = stepped(p, m, v, s, a.eps);
+    p = stepped(p, s.step_size * (m / madd(sqrtf(v), s.inv_bc2, a.eps)), s.lr_wd);
 }
 
 __device__ __forceinline__ double larger(double p, double q) { return p != p ? p : (q != q || q > p) ? q : p; }     // NaN wins
@@ -309,7 +308,7 @@ template <bool FULL> __device__ __forceinline__ void adamw8_run(Run8& r, const A
         r.cv |= cv << (8 * j);
         // fp32, the chip's own root and reciprocal: an ulp each, under 16 u of the update all told
         const float d = madd(__builtin_amdgcn_sqrtf((float)(v[j] * up)), down, a.eps);
-        r.x[j] -= madd(s.lr_wd, r.x[j], s.step_size * (float)m[j] * __builtin_amdgcn_rcpf(d));
+        r.x[j] = stepped(r.x[j], s.step_size * (float)m[j] * __builtin_amdgcn_rcpf(d), s.lr_wd);
     }
 }
 

@@ -347,6 +347,25 @@ def test_values_that_are_not_finite(bits):
         assert bool(torch.isfinite(p[fine]).all()) and not bool(torch.isfinite(p[300]))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("decay", [0.0, 0.1])
+def test_parameters_that_are_not_finite(bits, dtype, decay):
+    """inf (1 - lr wd) - update is inf, NaN stays NaN, and a half-precision parameter that a step carries over the edge is inf: as torch's"""
+    from remixfusion_amd.optim import AdamW
+    x = torch.full((600,), 1.0, device="cuda")
+    x[3], x[300], x[301], x[599] = math.inf, -math.inf, math.nan, 65000.0
+    p, q = (torch.nn.Parameter(x.to(DTYPES[dtype])) for _ in range(2))
+    p.grad, q.grad = (torch.full_like(p, -0.5) for _ in range(2))
+    lr = 2000.0 if dtype == "f16" else 0.01                     # 65000 + 2000 is no fp16
+    a, b = AdamW([p], lr=lr, weight_decay=decay / lr, state_bits=bits), torch.optim.AdamW([q], lr=lr, weight_decay=decay / lr, foreach=False)
+    for _ in range(2):
+        a.step(); b.step()
+        assert torch.equal(torch.isnan(p), torch.isnan(q)) and torch.equal(torch.isinf(p), torch.isinf(q))
+        assert torch.equal(torch.sign(p.detach()).nan_to_num(9.0), torch.sign(q.detach()).nan_to_num(9.0))
+    assert math.isinf(float(p.detach()[3])) and math.isinf(float(p.detach()[300])) and bool(torch.isinf(p[599])) == (dtype == "f16" and decay == 0.0)
+
+
 def test_eight_bits_over_the_whole_range():
     """gradients from the smallest subnormal to the largest finite number, runs of zeros, runs of one value"""
     from remixfusion_amd.optim import AdamW
