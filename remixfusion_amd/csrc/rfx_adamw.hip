@@ -12,7 +12,7 @@ namespace rfx {
 
 constexpr int AW_THREADS = 256;
 // Elements per block: four a thread, one run of the 8-bit form a wave.  Small blocks fill the chip early and leave no tail: against 4096
-// elements, 135 000 parameters in 8 bits step in 5 us instead of 9, and 41.5 million in 32 bits in 194 us instead of 206.
+// elements, 135 000 parameters in 8 bits step in 5 us instead of 9, and 41.5 million in 32 bits in 191 us instead of 206.
 constexpr int AW_PIECE = AW_THREADS * 4;
 constexpr int AW_TENSORS = 48;          // descriptors per launch: the kernel's arguments stay under 4 KB
 constexpr int AW_GROUPS = 8;
@@ -124,6 +124,7 @@ __device__ __forceinline__ float stepped(float p, float update, float lr_wd) {
 }
 
 // ---- 32-bit moments: fp32 throughout ------------------------------------------------------------------------------------------
+// Bound by HBM: 28 bytes an fp32 element, 41.5 million in 189 us = 6.1 TB/s (a large copy: 5.4).
 __device__ __forceinline__ void adamw_one(float& p, float g, float& m, float& v, const AwGroup& a, const AwStep& s, float c) {
     const float c1 = (float)a.c1, c2 = (float)a.c2, b1 = (float)a.b1, b2 = (float)a.b2;
     g *= c;
@@ -225,6 +226,11 @@ __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(const AwArgs k) {
 //           of two that is a constant of the run (beta goes into it: a product with a power of two is exact);
 //   encode: the moment times the inverse power of two, rounded to fp32 (subnormals included), leaves 20 bits below the format's
 //           last place: 16 random bits (and half of their unit) are added, and the upper bits are the code.
+// Why at random: one step moves an average by (1 - beta) of its distance -- a thousandth for beta2 = 0.999 -- and the formats' places
+// are an eighth apart; to nearest, the average would stand still.  Why second moments never become 0: m / eps would be a leap.
+// 16 bytes an fp32 element and 72 vector instructions: 41.5 million in 105-111 us = 6.0-6.3 TB/s; below some millions, where all of it
+// stays in the caches, the instructions bound it (3 million fp16 parameters, 30 MB: 12 us).  The codes are read and written through the
+// caches also where the rest goes past them: four bytes a lane, they share their lines with other waves.
 __device__ __forceinline__ double pow2(int e) { return __longlong_as_double((long long)(e + 1023) << 52); }
 
 template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
@@ -438,7 +444,9 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_moments_kernel(const MomArgs
 // ---- global norm --------------------------------------------------------------------------------------------------------------
 // One block per CU at most (16 waves, four loads of each in flight: enough to draw what HBM gives), so that there are never more
 // partial results than the blocks that read them join with one load a thread.  Each block has one piece, in whole rounds of its four
-// loads: 166 MB in 33 us; eight smaller pieces a block, dealt in turn, 35 us, eight loads in flight 40.
+// loads: 166 MB in 30 us (5.5 TB/s, what a large copy reaches); eight smaller pieces a block, dealt in turn, cost 2 us more, eight loads in
+// flight 6.  fp64 sums: no square of an fp32 number overflows or vanishes there, and the order -- pieces, lanes, waves, blocks -- is
+// fixed by the sizes alone.
 constexpr int GN_TENSORS = 128;
 constexpr int GN_THREADS = 1024;
 constexpr int64_t GN_ROUND = 4 * GN_THREADS;       // elements: one float4 a thread
@@ -508,7 +516,7 @@ __global__ __launch_bounds__(JOIN) void grad_norm_join_kernel(const double* part
 }
 
 // the norm's pieces on the blocks that the norm had them on: what an XCD's L2 still holds of a small set is found there (1.6 million
-// gradients 5.0 us, in pieces of another size 7.4)
+// gradients 5.8 us, in pieces of another size 7.4)
 template <typename T> __device__ __forceinline__ void scale_piece(T* g, int len, float c) {
     int done = 0;
     if (((uintptr_t)g & (4 * sizeof(T) - 1)) == 0) {
@@ -536,8 +544,9 @@ __global__ __launch_bounds__(GN_THREADS) void grad_scale_kernel(const GnArgs k) 
 static int elem_bytes(int dtype) { return dtype == RFX_F32 ? 4 : 2; }
 
 // From this much memory on (parameters, gradients, moments) the step's loads and stores go past the caches.
-// Measured, us a step (plain loads and stores / past the caches): 26 MB of fp32 tensors stepped again and again 9.5 / 11.6, 64 MB 19.6 / 25,
-// 128 MB 46 / 43, 665 MB 222 / 204; behind other work on 256 MB, as in a training loop, 16 MB 13.8 / 8.1, 64 MB 44 / 26, 128 MB 68 / 44.
+// Measured, us a step (plain loads and stores / past the caches), sets of fp32 tensors stepped again and again: 26 MB 9.6 / 11.0, 64 MB
+// 19 / 22, 128 MB 43 / 39, 664 MB 217 / 191; behind other work on 256 MB, as in a training loop: 16 MB 13.6 / 7.6, 64 MB 37 / 22, 128 MB
+// 64 / 40.  What is stepped next to nothing else stays in the caches under this size, and the larger sets gain either way.
 constexpr int64_t STREAM_BYTES = 64 << 20;
 static int64_t pieces_of(int64_t n) { return (n + AW_PIECE - 1) / AW_PIECE; }
 constexpr int64_t AW_BLOCKS = 0xffffffffLL / AW_THREADS;                   // of a launch: its threads are counted in 32 bits
