@@ -10,6 +10,13 @@ import torch
 from remixfusion_amd import _lib as L
 
 
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    from remixfusion_amd.build import build_host, build_library
+    build_library()
+    build_host()
+
+
 def _pair(**kw):
     from remixfusion_amd.optim import AdamW
     p = torch.nn.Parameter(torch.linspace(-1, 1, 12).reshape(3, 4).clone())
