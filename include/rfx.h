@@ -748,8 +748,8 @@ typedef struct rfx_adamw_tensor {
     void*        exp_avg_sq;            /* dev [n]: likewise                                                        */
     int8_t*      exponents;             /* dev [2][ceil(n / RFX_ADAMW_BLOCK)]: of exp_avg, then of exp_avg_sq (8 only) */
     float*       master;                /* dev [n] or NULL: the parameter in fp32, which is stepped in place of it    */
-    float*       step_dev;              /* dev [1] or NULL: the step count on the device (read, raised by one: for a   */
-                                        /* captured call); NULL: group.step                                         */
+    float*       step_dev;              /* dev [1] or NULL: this tensor's own step count on the device (read, raised by */
+                                        /* one: for a captured call); NULL: group.step                              */
     int64_t      n;
     int32_t      group;                 /* which of `groups`                                                        */
     uint32_t     index;                 /* of the parameter in its optimizer: keeps the tensors' roundings apart      */

@@ -103,7 +103,7 @@ class Plan {
 
     static Settings settings_of(PyObject* g) {
         const Keys& k = keys();
-        return {PyLong_AsLong(item(g, k.state_bits)), PyObject_IsTrue(item(g, k.master_weights)) == 1, PyObject_IsTrue(item(g, k.capturable)) == 1};
+        return {(long)number(item(g, k.state_bits)), PyObject_IsTrue(item(g, k.master_weights)) == 1, PyObject_IsTrue(item(g, k.capturable)) == 1};
     }
 
 public:
@@ -233,7 +233,7 @@ private:
                 e.beta2 = number(py::object(py::reinterpret_borrow<py::object>(betas)[py::int_(1)]).ptr());
                 e.eps = number(item(g, k.eps));
                 e.weight_decay = number(item(g, k.weight_decay));
-                e.seed = (uint32_t)PyLong_AsUnsignedLongMask(item(g, k.seed));
+                e.seed = (uint32_t)(int64_t)number(item(g, k.seed));
                 e.state_bits = (int32_t)settings_[gi].state_bits;
                 e.maximize = PyObject_IsTrue(item(g, k.maximize)) == 1;
                 e.step = step;

@@ -296,7 +296,7 @@ class AdamW(torch.optim.AdamW):
             group.setdefault(key, value)
         if group["state_bits"] not in (8, 32):
             raise ValueError(f"state_bits is 32 or 8: {group['state_bits']}")
-        if not isinstance(group["seed"], int) or not 0 <= group["seed"] < 1 << 32:
+        if group["seed"] != int(group["seed"]) or not 0 <= group["seed"] < 1 << 32:
             raise ValueError(f"seed is a whole number of 32 bits: {group['seed']}")
         super().add_param_group(group)
         ids = [id(p) for p in self.param_groups[-1]["params"]]

@@ -275,6 +275,26 @@ def test_many_tensors_clipped():
             assert float((p.grad.double() - g.double() / (want + 1e-6)).abs().max()) <= 3 * U * 8
 
 
+def test_numbers_of_other_types_in_the_groups():
+    """what a configuration file or numpy makes of the settings: 8.0 is 8, and a scalar is a float"""
+    from remixfusion_amd.optim import AdamW
+    ps = [torch.nn.Parameter(torch.linspace(-1, 1, 777, device="cuda")) for _ in range(2)]
+    a = AdamW([ps[0]], lr=np.float32(0.25), betas=(0.5, 0.75), eps=1e-8, weight_decay=0, state_bits=8.0, seed=3.0, master_weights=0, maximize=1)
+    b = AdamW([ps[1]], lr=0.25, betas=(0.5, 0.75), weight_decay=0.0, state_bits=8, seed=3, maximize=True)
+    for p, o in zip(ps, (a, b)):
+        p.grad = torch.ones_like(p)
+        o.step(); o.step()
+    assert torch.equal(ps[0], ps[1]) and torch.equal(a.state[ps[0]]["exp_avg"], b.state[ps[1]]["exp_avg"])
+    a.param_groups[0]["lr"] = None
+    with pytest.raises(TypeError):
+        a.step()
+    a.param_groups[0]["lr"] = 0.25
+    del a.param_groups[0]["eps"]
+    with pytest.raises(KeyError):
+        a.step()
+    assert torch.equal(ps[0], ps[1]) and float(a.state[ps[0]]["step"]) == 2.0
+
+
 def test_what_autograd_and_others_notice():
     """a step and a clipping raise the versions of what they write; a count that two parameters share is not raised twice"""
     from remixfusion_amd.optim import AdamW, clip_grad_norm_
