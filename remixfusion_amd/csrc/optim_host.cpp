@@ -4,7 +4,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
-#include <algorithm>
+#include <optional>
 #include <vector>
 #include "../../include/rfx.h"
 
@@ -71,6 +71,25 @@ const Keys& keys() { static const Keys* k = new Keys; return *k; }
 void written(const at::Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
+
+// fp32 tensor of these sizes and strides in `flat`'s memory, without the dispatcher's round that as_strided() makes
+py::object part_of(const at::Tensor& flat, int64_t at, at::IntArrayRef sizes, at::IntArrayRef strides) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(), flat.dtype());
+    impl->set_storage_offset(at);
+    impl->set_sizes_and_strides(sizes, strides);
+    return py::reinterpret_steal<py::object>(THPVariable_Wrap(at::Tensor(std::move(impl))));
+}
+
+// a call's workspace behind the 16 bytes whose first hold the norm that it returns
+struct Workspace {
+    at::Tensor memory;
+    size_t bytes;
+    Workspace(size_t n, at::Device device)
+        : memory(at::empty({4 + (int64_t)(n + 3) / 4}, at::TensorOptions().dtype(at::kFloat).device(device))), bytes(n) {}
+    float* norm() const { return static_cast<float*>(memory.data_ptr()); }
+    void* rest() const { return norm() + 4; }
+    py::object norm_tensor() const { return part_of(memory, 0, {}, {}); }
+};
 
 // what a step's outcome is to the caller: a negative status of librfx, or one of these
 enum Outcome { DONE = 0, STALE = 1, OTHER_ORDER = 2 };
@@ -248,25 +267,19 @@ private:
             }
             rows[i].group = (int32_t)at;
         }
-        py::object norm = py::none();
-        at::Tensor ws;
-        float* norm32 = nullptr;
-        const size_t bytes = limit >= 0.0 || counted_ ? rfx.adamw_workspace_bytes((int)n) : 0;
-        if (limit >= 0.0) {
+        const bool clipped = limit >= 0.0;
+        std::optional<Workspace> ws;
+        if (clipped || counted_) ws.emplace(rfx.adamw_workspace_bytes((int)n), device_);
+        if (clipped)
             for (size_t i = 0; i < n; ++i) grads_[i].grad = const_cast<void*>(rows[i].grad);
-            at::Tensor out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device_));
-            norm32 = static_cast<float*>(out.data_ptr());
-            norm = py::reinterpret_steal<py::object>(THPVariable_Wrap(out));
-        }
-        if (bytes) ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(device_));
-        const int rc = rfx.adamw_step(rows.data(), (int)n, groups_.data(), (int)groups_.size(), limit >= 0.0 ? grads_.data() : nullptr, limit, norm32,
-                                      bytes ? ws.data_ptr() : nullptr, bytes, (rfx_stream)stream);
+        const int rc = rfx.adamw_step(rows.data(), (int)n, groups_.data(), (int)groups_.size(), clipped ? grads_.data() : nullptr, limit,
+                                      clipped ? ws->norm() : nullptr, ws ? ws->rest() : nullptr, ws ? ws->bytes : 0, (rfx_stream)stream);
         if (rc != RFX_OK) return py::int_(rc);
         for (size_t i = 0; i < n; ++i) {
             if (counts_[i]) *counts_[i] += 1.f;
             written(tensor(params_[i].ptr()));
         }
-        return norm;
+        return clipped ? ws->norm_tensor() : py::none();
     }
 };
 
@@ -288,25 +301,14 @@ py::object clip(const py::list& parameters, int kind, double limit, int device, 
         rows.push_back(r);
     }
     if (rows.empty()) return py::int_((int)OTHER_ORDER);
-    const size_t bytes = rfx.grad_norm_workspace_bytes((int)rows.size());
-    at::Tensor ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
-    at::Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
-    const int rc = rfx.grad_clip(rows.data(), (int)rows.size(), kind, limit, static_cast<float*>(norm.data_ptr()), ws.data_ptr(), bytes,
-                                 (rfx_stream)stream);
+    const Workspace ws(rfx.grad_norm_workspace_bytes((int)rows.size()), dev);
+    const int rc = rfx.grad_clip(rows.data(), (int)rows.size(), kind, limit, ws.norm(), ws.rest(), ws.bytes, (rfx_stream)stream);
     if (rc != RFX_OK) return py::int_(rc);
     for (const auto& o : parameters) {
         const at::Tensor& g = tensor(o.ptr()).grad();
         if (g.defined()) written(g);
     }
-    return py::reinterpret_steal<py::object>(THPVariable_Wrap(norm));
-}
-
-// fp32 tensor of `like`'s sizes and strides in `flat`'s memory, without the dispatcher's round that as_strided() makes
-py::object part_of(const at::Tensor& flat, int64_t at, const at::Tensor& like) {
-    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(), flat.dtype());
-    impl->set_storage_offset(at);
-    impl->set_sizes_and_strides(like.sizes(), like.strides());
-    return py::reinterpret_steal<py::object>(THPVariable_Wrap(at::Tensor(std::move(impl))));
+    return ws.norm_tensor();
 }
 
 // the moments of all parameters in fp32: the state's own tensors where they are held in 32 bits, the codes' values where in 8
@@ -360,8 +362,8 @@ py::object moments(const py::list& param_groups, const py::dict& state, int devi
         for (size_t i = 0; i < rows.size(); ++i) {
             rows[i].out_avg = base + at;
             rows[i].out_avg_sq = base + total + at;
-            avg[codes[i].first] = part_of(flat, at, codes[i].second);
-            avg_sq[codes[i].first] = part_of(flat, total + at, codes[i].second);
+            avg[codes[i].first] = part_of(flat, at, codes[i].second.sizes(), codes[i].second.strides());
+            avg_sq[codes[i].first] = part_of(flat, total + at, codes[i].second.sizes(), codes[i].second.strides());
             at += (rows[i].n + 3) & ~(int64_t)3;
         }
         const int rc = rfx.adamw_moments(rows.data(), (int)rows.size(), (rfx_stream)stream);
