@@ -461,8 +461,13 @@ struct GnArgs {
 };
 static_assert(sizeof(GnArgs) <= 4096, "kernel arguments");
 
+// a lane's four neighbours wherever they start: the sums' order must not depend on an address
+template <typename T> __device__ __forceinline__ f4 load4_at(const T* p) {
+    typedef T any4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    return widen((vec4<T>)*reinterpret_cast<const any4*>(p));
+}
+
 template <typename T, bool MAX> __device__ __forceinline__ void norm_piece(const T* g, int len, double& sum, uint32_t& big) {
-    int done = 0;
     const auto one = [&](float x) {
         if (MAX) { const uint32_t u = __float_as_uint(x) & 0x7fffffffU; big = big > u ? big : u; }      // integers order NaN above all
         else { const double d = (double)x; sum = fma(d, d, sum); }
@@ -471,16 +476,14 @@ template <typename T, bool MAX> __device__ __forceinline__ void norm_piece(const
 #pragma unroll
         for (int j = 0; j < 4; ++j) one(x[j]);
     };
-    if (((uintptr_t)g & (4 * sizeof(T) - 1)) == 0) {
-        done = len & ~3;
-        int i = threadIdx.x * 4;
-        for (; i + 3 * GN_THREADS * 4 < done; i += 4 * GN_THREADS * 4) {
-            const f4 a = load4(g + i), b = load4(g + i + GN_THREADS * 4), c = load4(g + i + 2 * GN_THREADS * 4), d = load4(g + i + 3 * GN_THREADS * 4);
-            four(a); four(b); four(c); four(d);
-        }
-        for (; i < done; i += GN_THREADS * 4) four(load4(g + i));
+    const int done = len & ~3;
+    int i = threadIdx.x * 4;
+    for (; i + 3 * GN_THREADS * 4 < done; i += 4 * GN_THREADS * 4) {
+        const f4 a = load4_at(g + i), b = load4_at(g + i + GN_THREADS * 4), c = load4_at(g + i + 2 * GN_THREADS * 4), d = load4_at(g + i + 3 * GN_THREADS * 4);
+        four(a); four(b); four(c); four(d);
     }
-    for (int i = done + threadIdx.x; i < len; i += GN_THREADS) one((float)g[i]);
+    for (; i < done; i += GN_THREADS * 4) four(load4_at(g + i));
+    for (i = done + threadIdx.x; i < len; i += GN_THREADS) one((float)g[i]);
 }
 
 template <bool MAX>

@@ -1028,3 +1028,23 @@ def test_adam_with_decoupled_decay_is_not_stepped_as_l2():
         p.grad = q.grad = torch.full((100,), 0.25, device="cuda")
         ours.step(); ref.step()
     assert float((p - q).detach().abs().max()) <= 1e-6
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES.values()), ids=list(DTYPES))
+@pytest.mark.parametrize("n", [3, 4099, 70001, 3000003])
+def test_the_norm_does_not_depend_on_addresses(dtype, n):
+    """all 64 bits of the norm: the order of its sum is one of sizes, not of where the gradients start"""
+    from remixfusion_amd import _lib
+    lib = _lib.load()
+    g = (torch.randn(n, generator=torch.Generator().manual_seed(n)) * 0.3).to(dtype).cuda()
+    ws = torch.empty(lib.rfx_grad_norm_workspace_bytes(1) // 8, dtype=torch.float64, device="cuda")
+    seen = []
+    for first in (0, 1, 2, 3, 5):
+        at = torch.zeros(n + 8, dtype=dtype, device="cuda")[first:first + n].copy_(g)
+        clip = torch.empty(2, dtype=torch.float64, device="cuda")
+        row = (_lib.GradTensor * 1)(_lib.GradTensor(at.data_ptr(), n, _lib.DTYPES[dtype], 0))
+        _lib.check(lib.rfx_grad_norm(row, 1, 2, 1.0, clip.data_ptr(), None, ws.data_ptr(), ws.numel() * 8, _lib.stream_ptr(0)), "rfx_grad_norm")
+        seen.append(float(clip[0]))
+    assert len(set(seen)) == 1, seen
+    want = math.sqrt(float((g.cpu().double() ** 2).sum()))
+    assert abs(seen[0] - want) <= 1e-12 * want
