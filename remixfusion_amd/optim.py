@@ -250,7 +250,8 @@ class AdamW(torch.optim.AdamW):
     master_weights  bfloat16 / float16 parameters are stepped in an fp32 copy, state[p]["master"], and rounded once.
     seed            of the 8-bit roundings.
     max_grad_norm   scale the gradients by min(1, max_grad_norm / (N + 1e-6)), N their global 2-norm, on the way into the moments: the
-                    gradients themselves stay as they are.  `grad_norm` is N of the last step (fp32 scalar on the device).
+                    gradients themselves stay as they are.  `grad_norm` is N of the last step (fp32 scalar on the device; None where
+                    it had no limit or no gradient).
     capturable      the step count lives on the device and lr may be a device scalar: step() can be captured into a graph (after one
                     step or prepare(), which create the state).  Without it a capture is refused.
 
@@ -470,6 +471,7 @@ class AdamW(torch.optim.AdamW):
                 other = out == _lib.host().OTHER_ORDER
         params = [p for g in self.param_groups for p in g["params"] if p.grad is not None]
         if not params:
+            self.grad_norm = None
             return loss
         if not any(p.is_cuda for p in params):
             self._cpu_step()
@@ -497,8 +499,7 @@ class AdamW(torch.optim.AdamW):
         if isinstance(out, int):
             _lib.check(min(out, 0), "rfx_adamw_step")
             return False
-        if out is not None:
-            self.grad_norm = out
+        self.grad_norm = out
         return True
 
     def _cpu_step(self):

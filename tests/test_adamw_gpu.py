@@ -1048,3 +1048,14 @@ def test_the_norm_does_not_depend_on_addresses(dtype, n):
     assert len(set(seen)) == 1, seen
     want = math.sqrt(float((g.cpu().double() ** 2).sum()))
     assert abs(seen[0] - want) <= 1e-12 * want
+
+
+def test_the_norm_is_that_of_the_last_step():
+    from remixfusion_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(9, device="cuda"))
+    opt = AdamW([p], max_grad_norm=1.0)
+    for limit, grad, want in ((1.0, 2.0, 6.0), (None, 2.0, None), (5.0, 1.0, 3.0), (5.0, None, None), (0.0, 1.0, 3.0)):
+        opt.max_grad_norm = limit
+        p.grad = None if grad is None else torch.full_like(p, grad)
+        opt.step()
+        assert opt.grad_norm is None if want is None else float(opt.grad_norm) == want
