@@ -341,6 +341,8 @@ class AdamW(torch.optim.AdamW):
                         self.state[p]["step"] = self.state[p]["step"].detach().clone()      # (raised in place: not in the dict that was given)
                     if p.is_cuda:
                         self._check_state(p, g)
+                    elif p.is_floating_point():              # (torch's step on the CPU wants them in the parameter's type)
+                        self.state[p].update({k: st[k].to(p) for k in ("exp_avg", "exp_avg_sq") if k in st and st[k].is_floating_point()})
 
     def _check_state(self, p, g):
         """brings a state that came from outside to the types and the memory order a step needs, or refuses it"""

@@ -58,6 +58,20 @@ def test_copies_and_state_dicts_keep_what_is_ours():
     assert len(avg) == 2 and avg[0].shape == (3, 4) and float(avg_sq[1].abs().sum()) == 0.0                  # no state yet: zeros
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_device_runs_state_steps_on_the_cpu(dtype):
+    """moments in fp32, as a device holds them whatever the parameter's type"""
+    from remixfusion_amd.optim import AdamW
+    p, q = (torch.nn.Parameter(torch.linspace(-1, 1, 12).to(dtype)) for _ in range(2))
+    ours, ref = AdamW([p], lr=0.05), torch.optim.AdamW([q], lr=0.05)
+    state = {"step": torch.tensor(3.0), "exp_avg": torch.full((12,), 0.3), "exp_avg_sq": torch.full((12,), 0.7)}
+    for o in (ours, ref):
+        o.load_state_dict({"state": {0: copy.deepcopy(state)}, "param_groups": ref.state_dict()["param_groups"]})
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    ours.step(); ref.step()
+    assert torch.equal(p.detach(), q.detach()) and float(ours.state[p]["step"]) == 4.0
+
+
 def test_what_has_no_cpu_path_is_refused():
     for kw in ({"state_bits": 8}, {"master_weights": True}, {"max_grad_norm": 1.0}):
         p, q, ours, ref = _pair(**kw)
