@@ -425,7 +425,7 @@ class AdamW(torch.optim.AdamW):
     def _build(self, every):
         """plans for (parameter, its place in the optimizer, its group): states made or checked, one plan per device"""
         capturing = torch.cuda.is_current_stream_capturing()
-        by_device, counts = {}, set()
+        by_device, held = {}, set()
         for entry in every:
             p, _, gi = entry
             g = self.param_groups[gi]
@@ -443,9 +443,11 @@ class AdamW(torch.optim.AdamW):
             else:
                 self._new_state(p, g)
             st = self.state[p]
-            if st["step"].data_ptr() in counts:                  # one count for several parameters: each raises its own
-                st["step"] = st["step"].clone()
-            counts.add(st["step"].data_ptr())
+            for key in ("step", "exp_avg", "exp_avg_sq", "exponents", "master"):     # each parameter writes its own: none is shared
+                if key in st and st[key].numel():
+                    if st[key].data_ptr() in held:
+                        st[key] = st[key].clone()
+                    held.add(st[key].data_ptr())
         self._plans = {dev: (_lib.host().Plan(part, self.param_groups, self.state), part) for dev, part in by_device.items()}
 
     def step(self, closure=None):

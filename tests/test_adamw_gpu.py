@@ -1059,3 +1059,33 @@ def test_the_norm_is_that_of_the_last_step():
         p.grad = None if grad is None else torch.full_like(p, grad)
         opt.step()
         assert opt.grad_norm is None if want is None else float(opt.grad_norm) == want
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_that_parameters_share_is_parted(bits):
+    """one set of moments (and master weights) given to two parameters, and one tensor as both moments: as if each had its own"""
+    from remixfusion_amd.optim import AdamW
+    n = 1000
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    kind = torch.uint8 if bits == 8 else torch.float32
+    m = torch.full((n,), 40, dtype=kind, device="cuda")
+    st = {"step": torch.tensor(2.0), "exp_avg": m, "exp_avg_sq": m, "master": torch.randn(n, device="cuda", generator=gen)}
+    if bits == 8:
+        st["exponents"] = torch.zeros(2, 4, dtype=torch.int8, device="cuda")
+    grads = [torch.randn(n, device="cuda", generator=gen).bfloat16() for _ in range(2)]
+    out = []
+    for share in (True, False):
+        ps = [torch.nn.Parameter(torch.zeros(n, device="cuda", dtype=torch.bfloat16)) for _ in range(2)]
+        opt = AdamW(ps, lr=0.1, state_bits=bits, master_weights=True)
+        own = {k: t.clone() for k, t in st.items()}
+        if share:
+            own["exp_avg_sq"] = own["exp_avg"]
+        opt.load_state_dict({"state": {i: dict(own) if share else {k: t.clone() for k, t in st.items()} for i in range(2)},
+                             "param_groups": opt.state_dict()["param_groups"]})
+        for _ in range(3):
+            for p, g in zip(ps, grads):
+                p.grad = g.clone()
+            opt.step()
+        out.append([t.clone() for p in ps for t in (p.detach(), *opt.state[p].values())])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
