@@ -422,6 +422,31 @@ class AdamW(torch.optim.AdamW):
         return out
 
     # ---- the step ---------------------------------------------------------------------------------------------------------
+    @staticmethod
+    def _part(st, held):
+        """a state whose tensors are none of those held already: each parameter writes its own"""
+        for key in ("step", "exp_avg", "exp_avg_sq", "exponents", "master"):
+            if key in st and st[key].numel():
+                if st[key].data_ptr() in held:
+                    st[key] = st[key].clone()
+                held.add(st[key].data_ptr())
+
+    def _as_captured(self, p, g, held):
+        """refuses a state that this step would have to make or bring over: every replay would do it again"""
+        st = self.state.get(p)
+        if not st:
+            raise _lib.RfxError("the state is created by the first step() or prepare(): call it before capturing")
+        before = dict(st)
+        try:
+            self._check_state(p, g)
+            self._part(st, held)
+            if any(t is not before.get(key) for key, t in st.items()):
+                raise _lib.RfxError("the state is not as a captured step needs it: call step() or prepare() before capturing")
+        except _lib.RfxError:
+            st.clear()
+            st.update(before)
+            raise
+
     def _build(self, every):
         """plans for (parameter, its place in the optimizer, its group): states made or checked, one plan per device"""
         capturing = torch.cuda.is_current_stream_capturing()
@@ -436,18 +461,14 @@ class AdamW(torch.optim.AdamW):
                 raise _lib.RfxError(f"parameters of type {p.dtype} are not supported: float32, bfloat16 or float16")
             if p.layout is not torch.strided or _overlaps_itself(p):
                 raise _lib.RfxError("a parameter whose elements share memory (an expanded tensor) or that is sparse is not supported")
+            if capturing:
+                self._as_captured(p, g, held)
+                continue
             if self.state.get(p):
                 self._check_state(p, g)
-            elif capturing:
-                raise _lib.RfxError("the state is created by the first step() or prepare(): call it before capturing")
             else:
                 self._new_state(p, g)
-            st = self.state[p]
-            for key in ("step", "exp_avg", "exp_avg_sq", "exponents", "master"):     # each parameter writes its own: none is shared
-                if key in st and st[key].numel():
-                    if st[key].data_ptr() in held:
-                        st[key] = st[key].clone()
-                    held.add(st[key].data_ptr())
+            self._part(self.state[p], held)
         self._plans = {dev: (_lib.host().Plan(part, self.param_groups, self.state), part) for dev, part in by_device.items()}
 
     def step(self, closure=None):

@@ -1089,3 +1089,45 @@ def test_a_state_that_parameters_share_is_parted(bits):
         out.append([t.clone() for p in ps for t in (p.detach(), *opt.state[p].values())])
     for a, b in zip(*out):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("what", ["order", "type", "count", "shared", "master"])
+def test_a_capture_does_not_bring_a_state_over(what):
+    """what an eager step would convert once, a graph would convert on every replay: refused, and nothing of the state is changed"""
+    from remixfusion_amd import _lib as L
+    from remixfusion_amd.optim import AdamW
+    p, q = (torch.nn.Parameter(torch.ones(6, 4, device="cuda", dtype=torch.bfloat16)) for _ in range(2))
+    opt = AdamW([p, q], capturable=True, master_weights=what == "master")
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    opt.step()
+    st = opt.state[q]
+    if what == "order":
+        st["exp_avg"] = torch.zeros(4, 6, device="cuda").t()
+    elif what == "type":
+        st["exp_avg_sq"] = st["exp_avg_sq"].double()
+    elif what == "count":
+        st["step"] = torch.tensor(1.0)
+    elif what == "shared":
+        st["exp_avg"] = opt.state[p]["exp_avg"]
+    else:
+        del st["master"]
+    torch.cuda.synchronize()
+    before = {x: {k: (t, t.clone()) for k, t in opt.state[x].items()} for x in (p, q)}
+    torch.cuda.synchronize()
+    with pytest.raises(L.RfxError):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    for x in (p, q):
+        assert set(opt.state[x]) == set(before[x])
+        for k, (t, value) in before[x].items():
+            assert opt.state[x][k] is t and torch.equal(t, value)
+    opt.step()                                                     # an eager one brings it over
+    torch.cuda.synchronize()
+    assert opt.state[q]["exp_avg"] is not opt.state[p]["exp_avg"]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float(opt.state[q]["step"]) == 3.0
