@@ -774,10 +774,10 @@ typedef struct rfx_grad_tensor {
     int32_t reserved;
 } rfx_grad_tensor;
 /* tensors / groups: host arrays of any length (read before the call returns); few launches for all of them.  Tensors of one
- * call that share parameter memory are stepped one after the other.  clip_grads: NULL, or the `count` gradients again, whose
- * 2-norm N is formed first: they enter the moments times min(1, max_norm / (N + 1e-6)) and stay as they are themselves; norm32
- * (dev [1] or NULL) gets N.  workspace: dev, 16-byte aligned, >= rfx_adamw_workspace_bytes(count) where a tensor has step_dev or
- * there are clip_grads, else NULL.                                                                                          */
+ * call that share parameter memory are stepped one after the other; nothing else that is written may be shared.  clip_grads:
+ * NULL, or the `count` gradients again, whose 2-norm N is formed first: they enter the moments times min(1, max_norm / (N + 1e-6))
+ * and stay as they are themselves; norm32 (dev [1] or NULL) gets N.  workspace: dev, 16-byte aligned, >=
+ * rfx_adamw_workspace_bytes(count) where a tensor has step_dev or there are clip_grads, else NULL.                          */
 size_t rfx_adamw_workspace_bytes(int count);
 int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_group* groups, int n_groups,
                    const rfx_grad_tensor* clip_grads, double max_norm, float* norm32, void* workspace, size_t workspace_bytes,

@@ -120,6 +120,9 @@ class Plan {
     at::Device device_;
     bool ordered_ = true, counted_ = false, host_counted_ = false;
 
+    // (a user may keep something of their own in a state)
+    static void* at_of(PyObject* o) { return THPVariable_Check(o) ? THPVariable_Unpack(o).data_ptr() : nullptr; }
+
     static Settings settings_of(PyObject* g) {
         const Keys& k = keys();
         return {(long)number(item(g, k.state_bits)), PyObject_IsTrue(item(g, k.master_weights)) == 1, PyObject_IsTrue(item(g, k.capturable)) == 1};
@@ -146,7 +149,7 @@ public:
             PyObject *key, *value;
             for (Py_ssize_t at = 0; PyDict_Next(st, &at, &key, &value);) {
                 parts_.push_back(py::reinterpret_borrow<py::object>(value));
-                part_ptr_.push_back(tensor(value).data_ptr());
+                part_ptr_.push_back(at_of(value));
             }
             rfx_adamw_tensor r{};
             r.param = p.data_ptr();
@@ -206,7 +209,7 @@ public:
             if (values_[at_value].ptr() != value) return py::int_((int)STALE);
         for (const auto& st : states_)
             for (Py_ssize_t at = 0; PyDict_Next(st.ptr(), &at, &key, &value); ++at_part)
-                if (at_part == parts_.size() || parts_[at_part].ptr() != value || tensor(value).data_ptr() != part_ptr_[at_part]) return py::int_((int)STALE);
+                if (at_part == parts_.size() || parts_[at_part].ptr() != value || at_of(value) != part_ptr_[at_part]) return py::int_((int)STALE);
         if (at_part != parts_.size()) return py::int_((int)STALE);
         if (other) return py::int_((int)OTHER_ORDER);
         return run(rows_, param_groups, limit, stream);

@@ -1131,3 +1131,14 @@ def test_a_capture_does_not_bring_a_state_over(what):
     graph.replay()
     torch.cuda.synchronize()
     assert float(opt.state[q]["step"]) == 3.0
+
+
+def test_a_state_may_hold_what_is_not_a_tensor():
+    from remixfusion_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p])
+    opt.step()
+    opt.state[p]["name"] = "decoder"
+    opt.step(); opt.step()
+    assert opt.state[p]["name"] == "decoder" and float(opt.state[p]["step"]) == 3.0
