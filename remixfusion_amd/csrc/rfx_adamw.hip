@@ -297,8 +297,16 @@ template <bool FULL> __device__ __forceinline__ void adamw8_run(Run8& r, const A
     r.e1 = run_exponent<1>(wave_max(h1));
     r.e2 = run_exponent<2>(wave_max(h2));
     const double i1 = pow2(-112 - r.e1), i2 = pow2(-96 - 2 * r.e2);
+    int e = r.e2;
+    if (e == -128) {                                                       // (a scalar) what is not finite has no say in its neighbours' step
+        uint32_t h = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if ((FULL || j < have) && u2[j] < 0x7ff00000U) h = h > u2[j] ? h : u2[j];
+        e = run_exponent<2>(wave_max(h));
+    }
     // the root is taken of v 2^(2 half), which no fp32 overflows and next to none underflows: squares of fp32 numbers do both
-    const int half = r.e2 < -50 ? 100 : 50 - r.e2;
+    const int half = e < -50 ? 100 : 50 - e;
     const double up = pow2(2 * half);
     const float down = s.inv_bc2 * __uint_as_float((uint32_t)(127 - half) << 23);
     r.cm = r.cv = 0;

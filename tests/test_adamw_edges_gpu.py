@@ -1,0 +1,79 @@
+"""remixfusion_amd.optim.AdamW and clip_grad_norm_ at their edges: runs that hold a value that is not finite, gradients near the end of
+fp32's range, parameters whose memory has gaps in any order, states and groups that came from outside.
+
+Oracle and tolerances: test_adamw_gpu.py (everything in 64 bits; u = 2^-24)."""
+import copy
+import gc
+import math
+import weakref
+
+import numpy as np
+import pytest
+import torch
+
+from test_adamw_gpu import DTYPES, SETTINGS, U, Ref, decode, half_eps, magnitudes, near
+
+pytestmark = pytest.mark.gpu
+
+
+def _finite_runs(st, ref, what):
+    """codes and exponents as the oracle's where a run holds finite values only; the exponent that says so where not"""
+    assert np.array_equal(st["exponents"].cpu().numpy(), np.stack([ref.e1, ref.e2])), (what, "exponents")
+    n = len(ref.cm)
+    fine = np.repeat(ref.e1 != -128, 256)[:n]
+    assert np.array_equal(st["exp_avg_sq"].cpu().numpy().reshape(-1)[fine], ref.cv[fine]), (what, "exp_avg_sq")
+    near(torch.from_numpy(decode(st["exp_avg"].cpu().numpy().reshape(-1), ref.e1, 15)), ref.m, 0.0, (what, "exp_avg"))
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("dtype,master", [("f32", False), ("bf16", False), ("f16", False), ("bf16", True)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_neighbours_of_a_value_that_is_not_finite_step(bad, dtype, master, offset):
+    """in the step that meets it, every other element of its run moves by the formula: large, small and zero gradients, whole runs and
+    a tensor's last one, one bad element and all but one"""
+    from remixfusion_amd.optim import AdamW
+    T = DTYPES[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(41)
+    n = 2048 + 77
+    init = torch.randn(n + offset, device="cuda", generator=gen).mul(0.3).to(T)
+    p = torch.nn.Parameter(init[offset:])
+    opt = AdamW([p], **SETTINGS[1], state_bits=8, master_weights=master, seed=9)
+    ref = Ref(p.detach().float().cpu().numpy(), 8, 0, 9)
+    for it in range(3):
+        g = magnitudes(n + offset, gen)
+        g[offset + 256:offset + 512] *= 1e-6                        # fp16: down to its subnormals
+        g[offset + 512:offset + 768] *= 1e3
+        g = g.to(T)[offset:]
+        if it == 2:
+            for i in (3, 300, 700, 1023, 2047, 2100):
+                g[i] = bad
+            g[1025:1280] = bad                                      # all of a run but its first
+        p.grad = g
+        opt.step()
+        tp, _, _ = ref.step(g.float().cpu().numpy(), **SETTINGS[1], half=U if master else half_eps(T))
+        st = opt.state[p]
+        _finite_runs(st, ref, it)
+        near(st["master"] if master else p, ref.p, tp, (it, "p"))
+        ref.p = (st["master"] if master else p.detach()).double().cpu().numpy()
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+def test_a_clipped_step_with_an_infinite_gradient_is_a_step_of_zeros(bad):
+    """the norm is infinite, the factor 0: all but the bad element step on by their moments alone"""
+    from remixfusion_amd.optim import AdamW
+    gen = torch.Generator(device="cuda").manual_seed(43)
+    p = torch.nn.Parameter(torch.randn(1500, device="cuda", generator=gen))
+    opt = AdamW([p], **SETTINGS[1], state_bits=8, seed=4, max_grad_norm=0.5)
+    ref = Ref(p.detach().cpu().numpy(), 8, 0, 4)
+    for it in range(2):
+        p.grad = magnitudes(1500, gen)
+        if it:
+            p.grad[700] = bad
+        norm = math.sqrt(float((p.grad.double() ** 2).sum()))
+        opt.step()
+        with np.errstate(invalid="ignore"):
+            tp, _, _ = ref.step(p.grad.cpu().numpy(), **SETTINGS[1], c=min(1.0, 0.5 / (norm + 1e-6)))
+        assert math.isinf(float(opt.grad_norm)) == bool(it)
+        _finite_runs(opt.state[p], ref, it)
+        near(p, ref.p, tp, (it, "p"))
+        ref.p = p.detach().double().cpu().numpy()
