@@ -43,7 +43,17 @@ struct AwGroup {
     AwStep s;
     float eps;
     float sign;                         // -1: maximize
+    int32_t wide;                       // 8 bits: byte of a run's second moments from which its update is formed in fp64
 };
+
+// Runs of 8-bit moments whose denominators fp32 does not hold.  Scaled by the run's largest (2^e), a root of v under 2^(e - 113) is not normal
+// there: it may be lost next to an eps that is 2^35 times as large (ten bits of it for 1 / sqrt(1 - b2^k)), else m / eps would be a leap.  And
+// the chip's reciprocal makes 0 of what would be under 2^-126: roots from 2^91 on, with room for the same ten bits and for lr m.  A run is wide
+// from roots of 2^28 on with eps = 1e-15, of 2^51 with 1e-8; all others pay a comparison of scalars (41.6 million parameters 162 us as before).
+static int wide_from(double eps) {
+    const int e = eps > 0.0 && eps < 0x1p100 ? ilogb(eps) + 113 - 35 : -128;
+    return e < -128 ? -128 : e < 91 ? e : 91;
+}
 
 // Where the clipping factor comes from: partial sums (maxima) of the norm that every wave joins for itself -- never more than four a
 // lane, out of L2, for a launch less -- or a factor that is there.  Neither: no clipping.
@@ -297,18 +307,11 @@ template <bool FULL> __device__ __forceinline__ void adamw8_run(Run8& r, const A
     r.e1 = run_exponent<1>(wave_max(h1));
     r.e2 = run_exponent<2>(wave_max(h2));
     const double i1 = pow2(-112 - r.e1), i2 = pow2(-96 - 2 * r.e2);
-    int e = r.e2;
-    if (e == -128) {                                                       // (a scalar) what is not finite has no say in its neighbours' step
-        uint32_t h = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if ((FULL || j < have) && u2[j] < 0x7ff00000U) h = h > u2[j] ? h : u2[j];
-        e = run_exponent<2>(wave_max(h));
-    }
-    // the root is taken of v 2^(2 half), which no fp32 overflows and next to none underflows: squares of fp32 numbers do both
-    const int half = e < -50 ? 100 : 50 - e;
+    // the root is taken of v 2^(2 half), which no fp32 overflows; what underflows there is nothing next to eps, or the run is wide
+    const int half = r.e2 < -50 ? 100 : 50 - r.e2;
     const double up = pow2(2 * half);
     const float down = s.inv_bc2 * __uint_as_float((uint32_t)(127 - half) << 23);
+    const bool wide = r.e2 == -128 || r.e2 >= a.wide;                      // (a scalar)
     r.cm = r.cv = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -320,9 +323,14 @@ template <bool FULL> __device__ __forceinline__ void adamw8_run(Run8& r, const A
         cv = cv > some ? cv : some;
         r.cm |= (cm | ((uint32_t)__double2hiint(m[j]) >> 24 & 128U)) << (8 * j);
         r.cv |= cv << (8 * j);
-        // fp32, the chip's own root and reciprocal: an ulp each, under 16 u of the update all told
-        const float d = madd(__builtin_amdgcn_sqrtf((float)(v[j] * up)), down, a.eps);
-        r.x[j] = stepped(r.x[j], s.step_size * (float)m[j] * __builtin_amdgcn_rcpf(d), s.lr_wd);
+        float update;
+        if (wide) {
+            update = (float)((double)s.step_size * m[j] / (sqrt(v[j]) * s.inv_bc2 + a.eps));
+        } else {                                                           // fp32, the chip's own root and reciprocal: an ulp each, under 16 u all told
+            const float d = madd(__builtin_amdgcn_sqrtf((float)(v[j] * up)), down, a.eps);
+            update = s.step_size * (float)m[j] * __builtin_amdgcn_rcpf(d);
+        }
+        r.x[j] = stepped(r.x[j], update, s.lr_wd);
     }
 }
 
@@ -805,7 +813,8 @@ int rfx_adamw_step(const rfx_adamw_tensor* tensors, int count, const rfx_adamw_g
                             AwGroup& a = k.group[gi];
                             a.b1 = g.beta1; a.c1 = 1.0 - g.beta1; a.b2 = g.beta2; a.c2 = 1.0 - g.beta2;
                             a.eps = (float)g.eps;
-                            if (g.state_bits == 8 && g.eps > 0.0 && a.eps < 1.17549435e-38f) a.eps = 1.17549435e-38f;    // rcp takes less for 0
+                            if (g.state_bits == 8 && g.eps > 0.0) a.eps = fmaxf(a.eps, 0x1p-126f);      // rcp takes less for 0
+                            a.wide = wide_from(a.eps);
                             a.sign = g.maximize ? -1.f : 1.f;
                             if (!counted) a.s = step_scalars(g.lr, g.beta1, g.beta2, g.weight_decay, (double)g.step, g.seed);
                             prep.g[gi] = {g.lr, g.beta1, g.beta2, g.weight_decay, g.lr_dev, g.seed};

@@ -77,3 +77,25 @@ def test_a_clipped_step_with_an_infinite_gradient_is_a_step_of_zeros(bad):
         _finite_runs(opt.state[p], ref, it)
         near(p, ref.p, tp, (it, "p"))
         ref.p = p.detach().double().cpu().numpy()
+
+
+@pytest.mark.parametrize("lr", [1e-3, 50.0])
+@pytest.mark.parametrize("eps", [1e-8, 1e-15, 1e-42])
+def test_eight_bit_steps_of_the_largest_gradients(eps, lr):
+    """roots of second moments beyond 2^126, whose reciprocals no normal fp32 holds, alone and next to small ones and zeros"""
+    from remixfusion_amd.optim import AdamW
+    top = float(np.finfo(np.float32).max)
+    rows = [np.full(256, top), np.full(256, -2.0 ** 126), np.full(256, 2.0 ** 127), np.geomspace(1e-3, 3e38, 256), -np.geomspace(1e30, 3.4e38, 256),
+            np.where(np.arange(256) % 3 == 0, 0.0, 3.3e38), np.full(256, 2.0 ** 100), np.full(256, 2.0 ** 64), np.geomspace(1e-10, 1.0, 256)]
+    g = np.concatenate(rows + [np.full(77, 1.5e38)]).astype(np.float32)
+    p = torch.nn.Parameter(torch.zeros(len(g), device="cuda"))
+    opt = AdamW([p], lr=lr, betas=(0.9, 0.999), eps=eps, state_bits=8, weight_decay=0.0, seed=5)
+    ref = Ref(np.zeros(len(g)), 8, 0, 5)
+    for it in range(3):
+        p.grad = torch.from_numpy(g).cuda()
+        opt.step()
+        tp, _, _ = ref.step(g, lr, (0.9, 0.999), eps, 0.0)
+        _finite_runs(opt.state[p], ref, it)
+        near(p, ref.p, tp, it)
+        ref.p = p.detach().double().cpu().numpy()
+        g = g * np.float32(0.5)
