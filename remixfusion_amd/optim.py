@@ -357,7 +357,7 @@ class AdamW(torch.optim.AdamW):
                 raise _lib.RfxError(f"{key} of shape {tuple(t.shape)} on {t.device} for a parameter of shape {tuple(p.shape)} on {p.device}")
             if (t.dtype == torch.uint8) != eight:
                 raise _lib.RfxError(f"{key} of type {t.dtype} for a group with state_bits={g['state_bits']}: moments are not converted on the way in")
-            if order is None and _dense(t) and not eight:
+            if order is None and _dense(t):                  # (8 bits: the exponents are those of its runs)
                 order = t
             fits = _dense(t) and (_same_memory_order(t, order) if order is not None else t.is_contiguous())
             if eight:

@@ -99,3 +99,68 @@ def test_eight_bit_steps_of_the_largest_gradients(eps, lr):
         near(p, ref.p, tp, it)
         ref.p = p.detach().double().cpu().numpy()
         g = g * np.float32(0.5)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype,master", [("f32", False), ("bf16", True)])
+@pytest.mark.parametrize("cut", ["columns", "permuted", "every other"])
+def test_a_parameter_with_gaps_in_any_order_is_planned_again(cut, dtype, master, bits):
+    """neither dense nor in row order: a step without its gradient, a group that joins, a saved state and prepare() all leave it as it is"""
+    from remixfusion_amd.optim import AdamW
+    T = DTYPES[dtype]
+
+    def view(t):
+        if cut == "columns":
+            return t[:, 3:53, 0].t()
+        if cut == "permuted":
+            return t[1:9, :20].permute(2, 0, 1)
+        return t[::2, 5:25, 1].t()
+
+    def run(part):
+        gen = torch.Generator(device="cuda").manual_seed(3)
+        wide = torch.randn(40, 64, 3, device="cuda", generator=gen).to(T)
+        p, q = torch.nn.Parameter(view(wide)), torch.nn.Parameter(torch.ones(700, device="cuda", dtype=T))
+        assert not p.is_contiguous() and p.stride()[-1] != 1
+        before, inside = wide.clone(), torch.zeros_like(wide, dtype=torch.bool)
+        view(inside).fill_(True)
+        make = lambda: AdamW([p], lr=0.01, state_bits=bits, master_weights=master, seed=2)           # noqa: E731
+        opt = make()
+        if part:
+            opt.prepare()
+            opt.prepare()
+        for it in range(5):
+            p.grad = torch.randn(p.shape, device="cuda", generator=gen).to(T)
+            opt.step()
+            if part and it == 1:
+                grad, p.grad = p.grad, None
+                opt.step()
+            if part and it == 2:
+                opt.add_param_group({"params": [q]})
+                q.grad = torch.ones_like(q)
+            if part and it == 3:
+                saved = copy.deepcopy(opt.state_dict())
+                opt = make()
+                opt.add_param_group({"params": [q]})
+                opt.load_state_dict(saved)
+        assert torch.equal(wide[~inside], before[~inside]) and not torch.equal(wide[inside], before[inside])
+        return [p.detach().clone()] + [opt.state[p][k].clone() for k in ("exp_avg", "exp_avg_sq")]
+
+    for a, b in zip(run(True), run(False)):
+        assert torch.equal(a, b)
+
+
+def test_eight_bit_moments_of_another_order_are_still_refused():
+    """codes whose runs lie otherwise than the parameter's, or that differ between the two moments"""
+    from remixfusion_amd import _lib as L
+    from remixfusion_amd.optim import AdamW
+    wide = torch.zeros(40, 64, device="cuda")
+    zeros = lambda: torch.zeros(40, 50, dtype=torch.uint8, device="cuda")                            # noqa: E731
+    turned = lambda: torch.zeros(50, 40, dtype=torch.uint8, device="cuda").t()                       # noqa: E731
+    gaps = lambda: torch.zeros(40, 64, dtype=torch.uint8, device="cuda")[:, 3:53]                    # noqa: E731
+    for p, m, v in ((torch.zeros(40, 50, device="cuda"), turned(), turned()), (torch.zeros(40, 50, device="cuda"), zeros(), turned()),
+                    (wide[:, 3:53], zeros(), turned()), (wide[:, 3:53], turned(), zeros()), (wide[:, 3:53], gaps(), gaps())):
+        opt = AdamW([torch.nn.Parameter(p)], state_bits=8)
+        with pytest.raises(L.RfxError):
+            opt.load_state_dict({"state": {0: {"step": torch.tensor(1.0), "exp_avg": m, "exp_avg_sq": v,
+                                               "exponents": torch.zeros(2, 8, dtype=torch.int8, device="cuda")}},
+                                 "param_groups": opt.state_dict()["param_groups"]})
