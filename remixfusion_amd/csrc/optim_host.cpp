@@ -56,13 +56,14 @@ double number(PyObject* o) {
 
 struct Keys {
     PyObject *params, *lr, *betas, *eps, *weight_decay, *seed, *state_bits, *maximize, *master_weights, *capturable, *step, *exp_avg,
-        *exp_avg_sq, *exponents, *master;
+        *exp_avg_sq, *exponents, *master, *amsgrad, *differentiable, *decoupled;
     Keys() {
         const auto make = [](const char* s) { return PyUnicode_InternFromString(s); };
         params = make("params"); lr = make("lr"); betas = make("betas"); eps = make("eps"); weight_decay = make("weight_decay");
         seed = make("seed"); state_bits = make("state_bits"); maximize = make("maximize"); master_weights = make("master_weights");
         capturable = make("capturable"); step = make("step"); exp_avg = make("exp_avg"); exp_avg_sq = make("exp_avg_sq");
-        exponents = make("exponents"); master = make("master");
+        exponents = make("exponents"); master = make("master"); amsgrad = make("amsgrad"); differentiable = make("differentiable");
+        decoupled = make("decoupled_weight_decay");
     }
 };
 const Keys& keys() { static const Keys* k = new Keys; return *k; }
@@ -115,7 +116,7 @@ class Plan {
     std::vector<rfx_adamw_tensor> rows_;
     std::vector<rfx_grad_tensor> grads_;
     std::vector<rfx_adamw_group> groups_;
-    struct Settings { long state_bits; bool master, capturable; };
+    struct Settings { long state_bits; bool master, capturable; double seed; bool refused; };      // refused: the caller's check says why
     std::vector<Settings> settings_;    // per parameter group
     at::Device device_;
     bool ordered_ = true, counted_ = false, host_counted_ = false;
@@ -123,9 +124,17 @@ class Plan {
     // (a user may keep something of their own in a state)
     static void* at_of(PyObject* o) { return THPVariable_Check(o) ? THPVariable_Unpack(o).data_ptr() : nullptr; }
 
+    static bool set(PyObject* g, PyObject* key, bool otherwise) {
+        PyObject* v = PyDict_GetItemWithError(g, key);
+        const int on = v ? PyObject_IsTrue(v) : otherwise;
+        if (on < 0 || (!v && PyErr_Occurred())) throw py::error_already_set();
+        return on == 1;
+    }
+
     static Settings settings_of(PyObject* g) {
         const Keys& k = keys();
-        return {(long)number(item(g, k.state_bits)), PyObject_IsTrue(item(g, k.master_weights)) == 1, PyObject_IsTrue(item(g, k.capturable)) == 1};
+        return {(long)number(item(g, k.state_bits)), PyObject_IsTrue(item(g, k.master_weights)) == 1, PyObject_IsTrue(item(g, k.capturable)) == 1,
+                number(item(g, k.seed)), set(g, k.amsgrad, false) || set(g, k.differentiable, false) || !set(g, k.decoupled, true)};
     }
 
 public:
@@ -187,7 +196,8 @@ public:
         for (size_t gi = 0; gi < settings_.size(); ++gi) {
             PyObject* g = PyList_GET_ITEM(param_groups.ptr(), (Py_ssize_t)gi);
             const Settings s = settings_of(g);
-            if (s.state_bits != settings_[gi].state_bits || s.master != settings_[gi].master || s.capturable != settings_[gi].capturable)
+            if (s.state_bits != settings_[gi].state_bits || s.master != settings_[gi].master || s.capturable != settings_[gi].capturable
+                || s.seed != settings_[gi].seed || s.refused)
                 return py::int_((int)STALE);
             PyObject* list = item(g, k.params);
             if (!PyList_Check(list)) return py::int_((int)STALE);

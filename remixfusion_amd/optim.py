@@ -255,7 +255,8 @@ class AdamW(torch.optim.AdamW):
     capturable      the step count lives on the device and lr may be a device scalar: step() can be captured into a graph (after one
                     step or prepare(), which create the state).  Without it a capture is refused.
 
-    moments() gives the moments as fp32 tensors.  amsgrad and differentiable are refused."""
+    moments() gives the moments as fp32 tensors.  amsgrad, differentiable and decoupled_weight_decay=False are refused (ValueError) however
+    a group comes by them: on construction, joining, loading, or set in place and stepped."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=False, *, maximize=False,
                  capturable=False, state_bits=32, master_weights=False, seed=0, max_grad_norm=None, differentiable=False,
@@ -291,14 +292,23 @@ class AdamW(torch.optim.AdamW):
             raise ValueError(f"max_grad_norm has to be None or a number >= 0: {value}")
         self.defaults["max_grad_norm"] = None if value is None else float(value)
 
-    def add_param_group(self, group):
-        own = self._own
-        for key, value in own.items():
-            group.setdefault(key, value)
+    @staticmethod
+    def _check_group(group):
+        for key in ("amsgrad", "differentiable"):
+            if group.get(key):
+                raise ValueError(f"remixfusion_amd.optim.AdamW has no {key}")
+        if not group.get("decoupled_weight_decay", True):
+            raise ValueError("remixfusion_amd.optim.AdamW decays weights apart from the gradient only")
         if group["state_bits"] not in (8, 32):
             raise ValueError(f"state_bits is 32 or 8: {group['state_bits']}")
         if group["seed"] != int(group["seed"]) or not 0 <= group["seed"] < 1 << 32:
             raise ValueError(f"seed is a whole number of 32 bits: {group['seed']}")
+
+    def add_param_group(self, group):
+        own = self._own
+        for key, value in own.items():
+            group.setdefault(key, value)
+        self._check_group(group)
         super().add_param_group(group)
         ids = [id(p) for p in self.param_groups[-1]["params"]]
         if len(set(ids)) != len(ids):
@@ -323,6 +333,8 @@ class AdamW(torch.optim.AdamW):
 
         def without_held(opt, d):                            # the last of the hooks: what it keeps from torch is put in below
             seen.append(d)
+            for g, own in zip(d["param_groups"], mine):
+                self._check_group({**own, **g, "decoupled_weight_decay": True})       # (as torch's AdamW: a dict of Adam fits)
             return {**d, "state": {i: {k: v for k, v in st.items() if k not in held} if isinstance(st, dict) else st
                                    for i, st in d["state"].items()}}
 
@@ -451,6 +463,8 @@ class AdamW(torch.optim.AdamW):
         """plans for (parameter, its place in the optimizer, its group): states made or checked, one plan per device"""
         capturing = torch.cuda.is_current_stream_capturing()
         by_device, held = {}, set()
+        for g in self.param_groups:                           # (whose settings may have been changed in place)
+            self._check_group(g)
         for entry in every:
             p, _, gi = entry
             g = self.param_groups[gi]
@@ -528,6 +542,8 @@ class AdamW(torch.optim.AdamW):
         return True
 
     def _cpu_step(self):
+        for g in self.param_groups:
+            self._check_group(g)
         if self.max_grad_norm is not None or any(g["state_bits"] != 32 or g["master_weights"] for g in self.param_groups):
             raise _lib.RfxError("8-bit moments, master weights and max_grad_norm need device parameters: there is no CPU path")
         torch_step = torch.optim.AdamW.step

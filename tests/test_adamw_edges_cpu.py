@@ -1,0 +1,63 @@
+"""remixfusion_amd.optim.AdamW and clip_grad_norm_ without a GPU: groups and states that come from outside, what a plan holds on to."""
+import copy
+
+import pytest
+import torch
+
+from remixfusion_amd import _lib as L
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    from remixfusion_amd.build import build_host, build_library
+    build_library()
+    build_host()
+
+
+def _param():
+    p = torch.nn.Parameter(torch.linspace(-1, 1, 12))
+    p.grad = torch.ones(12)
+    return p
+
+
+@pytest.mark.parametrize("group", [{"amsgrad": True}, {"differentiable": True}, {"state_bits": 16}, {"seed": -1}, {"seed": 1 << 32}, {"seed": 0.5}])
+def test_groups_that_are_refused_however_they_come(group):
+    """as a group that joins, as a loaded one, as one that was changed in place: nothing of the optimizer moves"""
+    from remixfusion_amd.optim import AdamW
+    p = _param()
+    opt = AdamW([p], lr=0.05)
+    opt.step()
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [_param()], **group})
+    assert len(opt.param_groups) == 1
+    saved = copy.deepcopy(opt.state_dict())
+    saved["param_groups"][0].update(group, lr=7.0)
+    moments = opt.state[p]["exp_avg"]
+    with pytest.raises(ValueError):
+        opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == 0.05 and opt.state[p]["exp_avg"] is moments
+    assert all(opt.param_groups[0].get(k) != v for k, v in group.items())
+    opt.param_groups[0].update(group)
+    before = p.detach().clone()
+    with pytest.raises((ValueError, L.RfxError)):
+        opt.step()
+    assert torch.equal(p.detach(), before) and float(opt.state[p]["step"]) == 1.0
+
+
+def test_a_run_with_amsgrad_is_not_resumed_without_it():
+    from remixfusion_amd.optim import AdamW
+    p, q = _param(), _param()
+    theirs = torch.optim.AdamW([q], amsgrad=True)
+    theirs.step()
+    opt = AdamW([p])
+    with pytest.raises(ValueError):
+        opt.load_state_dict(theirs.state_dict())
+    assert not opt.state and opt.param_groups[0]["amsgrad"] is False
+    for kind in (torch.optim.AdamW, torch.optim.Adam):          # as torch's AdamW takes them: the decay stays apart from the gradient
+        opt.load_state_dict(kind([_param()]).state_dict())
+        assert opt.param_groups[0]["decoupled_weight_decay"] is True
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [_param()], "decoupled_weight_decay": False})
+    opt.param_groups[0]["decoupled_weight_decay"] = False
+    with pytest.raises(ValueError):
+        opt.step()

@@ -164,3 +164,24 @@ def test_eight_bit_moments_of_another_order_are_still_refused():
             opt.load_state_dict({"state": {0: {"step": torch.tensor(1.0), "exp_avg": m, "exp_avg_sq": v,
                                                "exponents": torch.zeros(2, 8, dtype=torch.int8, device="cuda")}},
                                  "param_groups": opt.state_dict()["param_groups"]})
+
+
+@pytest.mark.parametrize("key,value", [("amsgrad", True), ("differentiable", True), ("decoupled_weight_decay", False), ("seed", -1), ("state_bits", 16)])
+def test_a_group_that_asks_for_another_algorithm_does_not_step(key, value):
+    """set in a group after a step was planned: refused, nothing moves"""
+    from remixfusion_amd import _lib as L
+    from remixfusion_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p])
+    opt.step()
+    before = p.detach().clone()
+    usual = opt.param_groups[0][key]
+    opt.param_groups[0][key] = value
+    for call in (opt.step, opt.prepare):
+        with pytest.raises((ValueError, L.RfxError)):
+            call()
+    assert torch.equal(p.detach(), before) and float(opt.state[p]["step"]) == 1.0
+    opt.param_groups[0][key] = usual
+    opt.step()
+    assert float(opt.state[p]["step"]) == 2.0
