@@ -325,6 +325,7 @@ class AdamW(torch.optim.AdamW):
                 g.setdefault(k, v)
 
     # ---- state ------------------------------------------------------------------------------------------------------------
+    @torch.no_grad()
     def load_state_dict(self, state_dict):
         """as torch's, but moments and master weights keep their own types (torch casts them to the parameter's); a dict of
         torch.optim.AdamW fits groups with 32-bit moments"""

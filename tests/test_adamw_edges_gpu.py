@@ -185,3 +185,22 @@ def test_a_group_that_asks_for_another_algorithm_does_not_step(key, value):
     opt.param_groups[0][key] = usual
     opt.step()
     assert float(opt.state[p]["step"]) == 2.0
+
+
+def test_a_loaded_state_hangs_on_no_graph():
+    """master weights made from the parameter on loading (a dict of torch's AdamW has none) are values: the optimizer can be copied"""
+    from remixfusion_amd.optim import AdamW
+    p, q = (torch.nn.Parameter(torch.linspace(-1, 1, 500, device="cuda").bfloat16()) for _ in range(2))
+    for x in (p, q):
+        x.grad = torch.ones_like(x)
+    theirs = torch.optim.AdamW([q], lr=0.1)
+    theirs.step()
+    opt = AdamW([p], lr=0.1, master_weights=True)
+    opt.load_state_dict(theirs.state_dict())
+    assert all(not t.requires_grad and t.grad_fn is None for t in opt.state[p].values())
+    twin = copy.deepcopy(opt)
+    opt.step()
+    r = twin.param_groups[0]["params"][0]
+    r.grad = torch.ones_like(r)
+    twin.step()
+    assert torch.equal(p, r) and torch.equal(opt.state[p]["master"], twin.state[r]["master"])
