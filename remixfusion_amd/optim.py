@@ -340,22 +340,31 @@ class AdamW(torch.optim.AdamW):
                                    for i, st in d["state"].items()}}
 
         hook = self.register_load_state_dict_pre_hook(without_held)
+        before = self.state, self.param_groups, self._plans, self.grad_norm
         try:
             super().load_state_dict(state_dict)
+            for g, saved, old in zip(self.param_groups, seen[0]["param_groups"], mine):
+                g.update({k: v for k, v in old.items() if k not in saved})
+                for i, p in zip(saved["params"], g["params"]):
+                    st = seen[0]["state"].get(i)
+                    if st:
+                        self._take(p, g, {k: st[k] for k in held if k in st})
+        except Exception:                                    # taken whole or not at all
+            self.state, self.param_groups, self._plans, self.grad_norm = before
+            raise
         finally:
             hook.remove()
-        for g, saved, old in zip(self.param_groups, seen[0]["param_groups"], mine):
-            g.update({k: v for k, v in old.items() if k not in saved})
-            for i, p in zip(saved["params"], g["params"]):
-                st = seen[0]["state"].get(i)
-                if st:
-                    self.state[p].update({k: st[k].to(device=p.device) for k in held if k in st})
-                    if isinstance(self.state[p].get("step"), torch.Tensor):
-                        self.state[p]["step"] = self.state[p]["step"].detach().clone()      # (raised in place: not in the dict that was given)
-                    if p.is_cuda:
-                        self._check_state(p, g)
-                    elif p.is_floating_point():              # (torch's step on the CPU wants them in the parameter's type)
-                        self.state[p].update({k: st[k].to(p) for k in ("exp_avg", "exp_avg_sq") if k in st and st[k].is_floating_point()})
+
+    def _take(self, p, g, held):
+        """the part of a loaded state that torch's loading was not to see"""
+        st = self.state[p]
+        st.update({k: t.to(device=p.device) for k, t in held.items()})
+        if isinstance(st.get("step"), torch.Tensor):
+            st["step"] = st["step"].detach().clone()         # (raised in place: not in the dict that was given)
+        if p.is_cuda:
+            self._check_state(p, g)
+        elif p.is_floating_point():                          # (torch's step on the CPU wants them in the parameter's type)
+            st.update({k: held[k].to(p) for k in ("exp_avg", "exp_avg_sq") if k in held and held[k].is_floating_point()})
 
     def _check_state(self, p, g):
         """brings a state that came from outside to the types and the memory order a step needs, or refuses it"""

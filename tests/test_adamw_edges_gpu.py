@@ -204,3 +204,27 @@ def test_a_loaded_state_hangs_on_no_graph():
     r.grad = torch.ones_like(r)
     twin.step()
     assert torch.equal(p, r) and torch.equal(opt.state[p]["master"], twin.state[r]["master"])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_state_changes_nothing(bits):
+    """load_state_dict takes a state whole or not at all"""
+    from remixfusion_amd import _lib as L
+    from remixfusion_amd.optim import AdamW
+    ps = [torch.nn.Parameter(torch.ones(n, device="cuda")) for n in (300, 40)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt = AdamW(ps, lr=0.1, state_bits=bits)
+    opt.step()
+    bad = copy.deepcopy(opt.state_dict())
+    bad["param_groups"][0]["lr"] = 7.0
+    bad["state"][0]["exp_avg"].fill_(1)
+    bad["state"][1]["exp_avg"] = bad["state"][1]["exp_avg"][:39]
+    before = {p: {k: (t, t.clone()) for k, t in opt.state[p].items()} for p in ps}
+    with pytest.raises(L.RfxError):
+        opt.load_state_dict(bad)
+    assert opt.param_groups[0]["lr"] == 0.1 and set(opt.state) == set(ps)
+    for p in ps:
+        assert all(opt.state[p][k] is t and torch.equal(t, value) for k, (t, value) in before[p].items())
+    opt.step()
+    assert [float(opt.state[p]["step"]) for p in ps] == [2.0, 2.0]
