@@ -349,6 +349,9 @@ class AdamW(torch.optim.AdamW):
                     st = seen[0]["state"].get(i)
                     if st:
                         self._take(p, g, {k: st[k] for k in held if k in st})
+            parted = set()
+            for p in (p for g in self.param_groups for p in g["params"] if p.is_cuda and self.state.get(p)):
+                self._part(self.state[p], parted)
         except Exception:                                    # taken whole or not at all
             self.state, self.param_groups, self._plans, self.grad_norm = before
             raise
@@ -445,13 +448,16 @@ class AdamW(torch.optim.AdamW):
 
     # ---- the step ---------------------------------------------------------------------------------------------------------
     @staticmethod
-    def _part(st, held):
+    def _tensors(st):
+        """(key, tensor) of what a step writes of a state"""
+        return [(k, st[k]) for k in ("step", "exp_avg", "exp_avg_sq", "exponents", "master") if isinstance(st.get(k), torch.Tensor) and st[k].numel()]
+
+    def _part(self, st, held):
         """a state whose tensors are none of those held already: each parameter writes its own"""
-        for key in ("step", "exp_avg", "exp_avg_sq", "exponents", "master"):
-            if key in st and st[key].numel():
-                if st[key].data_ptr() in held:
-                    st[key] = st[key].clone()
-                held.add(st[key].data_ptr())
+        for key, t in self._tensors(st):
+            if t.data_ptr() in held:
+                st[key] = t = t.clone()
+            held.add(t.data_ptr())
 
     def _as_captured(self, p, g, held):
         """refuses a state that this step would have to make or bring over: every replay would do it again"""
@@ -472,7 +478,8 @@ class AdamW(torch.optim.AdamW):
     def _build(self, every):
         """plans for (parameter, its place in the optimizer, its group): states made or checked, one plan per device"""
         capturing = torch.cuda.is_current_stream_capturing()
-        by_device, held = {}, set()
+        stepped = {p for p, _, _ in every}
+        by_device, held = {}, {t.data_ptr() for p, st in self.state.items() if p not in stepped and isinstance(st, dict) for _, t in self._tensors(st)}
         for g in self.param_groups:                           # (whose settings may have been changed in place)
             self._check_group(g)
         for entry in every:

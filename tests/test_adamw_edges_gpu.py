@@ -228,3 +228,38 @@ def test_a_refused_state_changes_nothing(bits):
         assert all(opt.state[p][k] is t and torch.equal(t, value) for k, (t, value) in before[p].items())
     opt.step()
     assert [float(opt.state[p]["step"]) for p in ps] == [2.0, 2.0]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_shared_state_is_parted_whatever_steps_first(bits):
+    """one set of moments loaded for two parameters whose gradients come in different steps"""
+    from remixfusion_amd.optim import AdamW
+    n = 1000
+    kind = torch.uint8 if bits == 8 else torch.float32
+    out = []
+    for share in (True, False):
+        gen = torch.Generator(device="cuda").manual_seed(4)
+        ps = [torch.nn.Parameter(torch.zeros(n, device="cuda", dtype=torch.bfloat16)) for _ in range(2)]
+        opt = AdamW(ps, lr=0.1, state_bits=bits, master_weights=True)
+        make = lambda: {"step": torch.tensor(2.0), "exp_avg": torch.full((n,), 40, dtype=kind, device="cuda"),             # noqa: E731
+                        "exp_avg_sq": torch.full((n,), 40, dtype=kind, device="cuda"), "master": torch.ones(n, device="cuda"),
+                        **({"exponents": torch.zeros(2, 4, dtype=torch.int8, device="cuda")} if bits == 8 else {})}
+        one = make()
+        opt.load_state_dict({"state": {i: one if share else make() for i in range(2)}, "param_groups": opt.state_dict()["param_groups"]})
+        for it in range(4):
+            for i, p in enumerate(ps):
+                p.grad = torch.randn(n, device="cuda", generator=gen).bfloat16() if it % 2 == i else None
+            opt.step()
+        out.append([t.clone() for p in ps for t in (p.detach(), *opt.state[p].values())])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+    # set by hand, between steps
+    p, q = (torch.nn.Parameter(torch.zeros(n, device="cuda")) for _ in range(2))
+    opt = AdamW([p, q], lr=0.1, state_bits=bits)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    opt.state[q] = dict(opt.state[p])
+    p.grad, q.grad = None, torch.ones_like(q)
+    held = {k: t.clone() for k, t in opt.state[p].items()}
+    opt.step()
+    assert all(torch.equal(held[k], t) for k, t in opt.state[p].items()) and float(opt.state[q]["step"]) == 2.0
