@@ -188,13 +188,14 @@ def _grad_rows(grads):
     return (_lib.GradTensor * len(grads))(*[_lib.GradTensor(g.data_ptr(), g.numel(), _lib.DTYPES[g.dtype], 0) for g in grads])
 
 
-def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
     """torch.nn.utils.clip_grad_norm_ as two passes of librfx kernels: the norm N of all gradients together (2-norm, summed in
     fp64 in an order that depends on sizes only, or the largest magnitude with norm_type=inf), then every gradient times
     min(1, max_norm / (N + 1e-6)) in place -- nothing is written where that is 1.  Returns N, an fp32 scalar on the gradients'
     device; the host does not wait for it unless error_if_nonfinite asks (RuntimeError before anything is scaled).  A factor that is
     not finite is applied as it is: an infinite norm makes zeros (and NaN of what was infinite), a NaN makes NaN.  One device;
-    float32 / bfloat16 / float16 gradients, mixed freely.  Gradients on the CPU take torch's own function."""
+    float32 / bfloat16 / float16 gradients, mixed freely.  Gradients on the CPU take torch's own function, and only there does
+    `foreach` (torch's choice between its own implementations) make a difference."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm, norm_type = float(max_norm), float(norm_type)
     if not max_norm >= 0.0:
@@ -210,7 +211,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     if not grads:
         return torch.tensor(0.0)
     if not any(g.is_cuda for g in grads):
-        return torch.nn.utils.clip_grad_norm_(parameters, max_norm, norm_type, error_if_nonfinite)
+        return torch.nn.utils.clip_grad_norm_(parameters, max_norm, norm_type, error_if_nonfinite, foreach)
     if norm_type not in (2.0, math.inf):
         raise _lib.RfxError(f"norm_type {norm_type}: only 2 and inf are supported")
     dev = grads[0].device

@@ -61,3 +61,10 @@ def test_a_run_with_amsgrad_is_not_resumed_without_it():
     opt.param_groups[0]["decoupled_weight_decay"] = False
     with pytest.raises(ValueError):
         opt.step()
+
+
+def test_clip_takes_torchs_arguments():
+    from remixfusion_amd.optim import clip_grad_norm_
+    for kw in ({"foreach": None}, {"foreach": False}, {"foreach": True}, {"error_if_nonfinite": True, "foreach": False, "norm_type": 3.0}):
+        p, q = _param(), _param()
+        assert torch.equal(clip_grad_norm_([p], 0.5, **kw), torch.nn.utils.clip_grad_norm_([q], 0.5, **kw)) and torch.equal(p.grad, q.grad)

@@ -263,3 +263,14 @@ def test_a_shared_state_is_parted_whatever_steps_first(bits):
     held = {k: t.clone() for k, t in opt.state[p].items()}
     opt.step()
     assert all(torch.equal(held[k], t) for k, t in opt.state[p].items()) and float(opt.state[q]["step"]) == 2.0
+
+
+def test_clip_takes_torchs_arguments():
+    from remixfusion_amd.optim import clip_grad_norm_
+    p, q = (torch.nn.Parameter(torch.zeros(5000, device="cuda")) for _ in range(2))
+    for foreach in (None, True, False):
+        for kw in ({"foreach": foreach}, {"norm_type": math.inf, "error_if_nonfinite": True, "foreach": foreach}):
+            p.grad = torch.linspace(-1, 2, 5000, device="cuda")
+            q.grad = p.grad.clone()
+            a, b = clip_grad_norm_([p], 0.5, **kw), torch.nn.utils.clip_grad_norm_([q], 0.5, **kw)
+            assert abs(float(a) - float(b)) <= 1e-5 * float(b) and float((p.grad - q.grad).abs().max()) <= 1e-6
