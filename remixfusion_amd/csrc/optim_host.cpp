@@ -108,8 +108,23 @@ struct Memory {                         // where a tensor was
 // What the descriptors of a step hold that stays the same from step to step: the parameters that have a gradient, on one device, and
 // their state.  Every step checks it against the optimizer's own lists; where anything moved, the caller builds another.
 class Plan {
-    std::vector<py::object> params_, states_, parts_, values_;
-    std::vector<void*> part_ptr_;
+    // A tensor of a state as it was, without keeping it alive: its impl's address is taken by no other while this weak reference lasts
+    struct Part {
+        c10::weak_intrusive_ptr<c10::TensorImpl> impl;
+        void* ptr;
+        int64_t n;
+        at::ScalarType dtype;
+        static void* at(const at::Tensor& t) { return t.has_storage() ? t.data_ptr() : nullptr; }
+        explicit Part(const at::Tensor& t) : impl(t.getIntrusivePtr()), ptr(at(t)), n(t.numel()), dtype(t.scalar_type()) {}
+        bool is(const at::Tensor& t) const {
+            return t.unsafeGetTensorImpl() == impl._unsafe_get_target() && at(t) == ptr && t.numel() == n && t.scalar_type() == dtype;
+        }
+    };
+
+    std::vector<py::object> params_;
+    std::vector<std::pair<PyObject*, PyObject*>> entries_;      // the optimizer's states: addresses only, that keep nothing alive
+    std::vector<PyObject*> states_;                             // the planned parameters' among them: looked into once all are found where they were
+    std::vector<Part> parts_;                           // (a user may keep something of their own in a state: only tensors count)
     std::vector<Memory> where_;
     std::vector<int> group_of_;
     std::vector<float*> counts_;        // host step counts; null: on the device
@@ -120,9 +135,6 @@ class Plan {
     std::vector<Settings> settings_;    // per parameter group
     at::Device device_;
     bool ordered_ = true, counted_ = false, host_counted_ = false;
-
-    // (a user may keep something of their own in a state)
-    static void* at_of(PyObject* o) { return THPVariable_Check(o) ? THPVariable_Unpack(o).data_ptr() : nullptr; }
 
     static bool set(PyObject* g, PyObject* key, bool otherwise) {
         PyObject* v = PyDict_GetItemWithError(g, key);
@@ -151,15 +163,13 @@ public:
             const at::Tensor &m = tensor(item(st, k.exp_avg)), &v = tensor(item(st, k.exp_avg_sq)), &step = tensor(item(st, k.step));
             device_ = p.device();
             params_.push_back(py::reinterpret_borrow<py::object>(t[0]));
-            states_.push_back(py::reinterpret_borrow<py::object>(st));
+            states_.push_back(st);
             where_.emplace_back(p);
             group_of_.push_back(group);
             ordered_ &= p.strides() == m.strides();
             PyObject *key, *value;
-            for (Py_ssize_t at = 0; PyDict_Next(st, &at, &key, &value);) {
-                parts_.push_back(py::reinterpret_borrow<py::object>(value));
-                part_ptr_.push_back(at_of(value));
-            }
+            for (Py_ssize_t at = 0; PyDict_Next(st, &at, &key, &value);)
+                if (THPVariable_Check(value)) parts_.emplace_back(THPVariable_Unpack(value));
             rfx_adamw_tensor r{};
             r.param = p.data_ptr();
             r.exp_avg = m.data_ptr();
@@ -181,7 +191,7 @@ public:
             grads_.push_back(gr);
         }
         PyObject *key, *value;
-        for (Py_ssize_t at = 0; PyDict_Next(state.ptr(), &at, &key, &value);) values_.push_back(py::reinterpret_borrow<py::object>(value));
+        for (Py_ssize_t at = 0; PyDict_Next(state.ptr(), &at, &key, &value);) entries_.emplace_back(key, value);
     }
 
     bool host_counted() const { return host_counted_; }
@@ -189,7 +199,7 @@ public:
     // the whole step where everything is as planned; else nothing has happened yet
     py::object step(const py::list& param_groups, const py::dict& state, double limit, uintptr_t stream) {
         const Keys& k = keys();
-        if (param_groups.size() != settings_.size() || (size_t)PyDict_Size(state.ptr()) != values_.size())
+        if (param_groups.size() != settings_.size() || (size_t)PyDict_Size(state.ptr()) != entries_.size())
             return py::int_((int)STALE);
         size_t n = 0, at_value = 0, at_part = 0;
         bool other = !ordered_;
@@ -216,10 +226,13 @@ public:
         if (n != params_.size()) return py::int_((int)STALE);
         PyObject *key, *value;
         for (Py_ssize_t at = 0; PyDict_Next(state.ptr(), &at, &key, &value); ++at_value)
-            if (values_[at_value].ptr() != value) return py::int_((int)STALE);
-        for (const auto& st : states_)
-            for (Py_ssize_t at = 0; PyDict_Next(st.ptr(), &at, &key, &value); ++at_part)
-                if (at_part == parts_.size() || parts_[at_part].ptr() != value || at_of(value) != part_ptr_[at_part]) return py::int_((int)STALE);
+            if (entries_[at_value].first != key || entries_[at_value].second != value) return py::int_((int)STALE);
+        for (PyObject* st : states_) {
+            if (!PyDict_Check(st)) return py::int_((int)STALE);
+            for (Py_ssize_t at = 0; PyDict_Next(st, &at, &key, &value);)
+                if (THPVariable_Check(value) && (at_part == parts_.size() || !parts_[at_part++].is(THPVariable_Unpack(value))))
+                    return py::int_((int)STALE);
+        }
         if (at_part != parts_.size()) return py::int_((int)STALE);
         if (other) return py::int_((int)OTHER_ORDER);
         return run(rows_, param_groups, limit, stream);

@@ -1,5 +1,7 @@
 """remixfusion_amd.optim.AdamW and clip_grad_norm_ without a GPU: groups and states that come from outside, what a plan holds on to."""
 import copy
+import gc
+import weakref
 
 import pytest
 import torch
@@ -68,3 +70,21 @@ def test_clip_takes_torchs_arguments():
     for kw in ({"foreach": None}, {"foreach": False}, {"foreach": True}, {"error_if_nonfinite": True, "foreach": False, "norm_type": 3.0}):
         p, q = _param(), _param()
         assert torch.equal(clip_grad_norm_([p], 0.5, **kw), torch.nn.utils.clip_grad_norm_([q], 0.5, **kw)) and torch.equal(p.grad, q.grad)
+
+
+def test_a_plan_keeps_no_state_alive():
+    """an optimizer's state that is cleared is freed, and no other tensor at its address is taken for it"""
+    p = _param()
+    state = {p: {"step": torch.zeros(()), "exp_avg": torch.zeros(12), "exp_avg_sq": torch.zeros(12), "name": "p"}}
+    groups = [dict(params=[p], state_bits=32, master_weights=False, capturable=False, seed=0)]
+    plan = L.host().Plan([(p, 0, 0)], groups, state)
+    seen = [weakref.ref(state[p][k]) for k in ("step", "exp_avg", "exp_avg_sq")]
+    state.clear()
+    gc.collect()
+    assert all(r() is None for r in seen)
+    state[p] = {"step": torch.zeros(()), "exp_avg": torch.zeros(12), "exp_avg_sq": torch.zeros(12), "name": "p"}
+    assert plan.step(groups, state, -1.0, 0) == L.host().STALE
+    state.clear()
+    assert plan.step(groups, state, -1.0, 0) == L.host().STALE
+    state[p] = None
+    assert plan.step(groups, state, -1.0, 0) == L.host().STALE

@@ -274,3 +274,28 @@ def test_clip_takes_torchs_arguments():
             q.grad = p.grad.clone()
             a, b = clip_grad_norm_([p], 0.5, **kw), torch.nn.utils.clip_grad_norm_([q], 0.5, **kw)
             assert abs(float(a) - float(b)) <= 1e-5 * float(b) and float((p.grad - q.grad).abs().max()) <= 1e-6
+
+
+def test_a_cleared_state_is_freed():
+    from remixfusion_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(1 << 20, device="cuda"))
+    p.grad = torch.ones_like(p)
+    torch.cuda.synchronize()
+    base = torch.cuda.memory_allocated()
+    opt = AdamW([p], lr=0.1)
+    opt.step()
+    opt.step()
+    held = weakref.ref(opt.state[p]["exp_avg"])
+    assert torch.cuda.memory_allocated() >= base + 2 * 4 * (1 << 20)
+    opt.state.clear()
+    gc.collect()
+    assert held() is None and torch.cuda.memory_allocated() < base + (1 << 20)
+    opt.step()
+    assert float(opt.state[p]["step"]) == 1.0
+    st = opt.state[p]                                              # a tensor that is cut down in place, or takes another's memory
+    from remixfusion_amd import _lib as L
+    before = p.detach().clone()
+    st["exp_avg"].data = st["exp_avg"].data[:100]
+    with pytest.raises(L.RfxError):
+        opt.step()
+    assert torch.equal(p.detach(), before)
