@@ -435,10 +435,12 @@ class AdamW(torch.optim.AdamW):
 
     def moments(self):
         """(exp_avg, exp_avg_sq) of all parameters, in their order, as fp32 tensors: the state's own tensors where moments are held
-        in 32 bits, the values of the codes where in 8, zeros where there is no state yet"""
+        in 32 bits, the values of the codes where in 8 (on a device), zeros where there is no state yet"""
         codes = [st["exp_avg"] for st in self.state.values() if st and st["exp_avg"].dtype is torch.uint8]
         if not codes:                                            # nothing to launch
             return _lib.host().moments(self.param_groups, self.state, -1, 0)
+        if not codes[0].is_cuda:
+            raise _lib.RfxError("8-bit moments are read on a device: there is no CPU path")
         index = codes[0].get_device()
         with _on(index):
             out = _lib.host().moments(self.param_groups, self.state, index, _lib.stream_ptr(index))

@@ -88,3 +88,16 @@ def test_a_plan_keeps_no_state_alive():
     assert plan.step(groups, state, -1.0, 0) == L.host().STALE
     state[p] = None
     assert plan.step(groups, state, -1.0, 0) == L.host().STALE
+
+
+def test_eight_bit_moments_on_the_cpu_say_what_they_need():
+    """a device run's state loaded without one: it can be kept and saved, its values are read on a device"""
+    from remixfusion_amd.optim import AdamW
+    p = _param()
+    opt = AdamW([p], state_bits=8)
+    codes = torch.arange(12, dtype=torch.uint8)
+    opt.load_state_dict({"state": {0: {"step": torch.tensor(3.0), "exp_avg": codes, "exp_avg_sq": codes.clone(),
+                                       "exponents": torch.zeros(2, 1, dtype=torch.int8)}}, "param_groups": opt.state_dict()["param_groups"]})
+    assert torch.equal(opt.state_dict()["state"][0]["exp_avg"], codes)
+    with pytest.raises(L.RfxError, match="device"):
+        opt.moments()
