@@ -140,8 +140,8 @@ _capturing = torch._C._cuda_isCurrentStreamCapturing if hasattr(torch._C, "_cuda
 
 
 def _same_memory_order(a, b):
-    """whether two tensors of one shape hold element i of memory for the same place (both dense, equal strides)"""
-    return a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous())
+    """whether two dense tensors of one shape hold element i of memory for the same place (a size-1 dimension's stride means nothing)"""
+    return a.stride() == b.stride() or a.numel() == 0 or all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1)
 
 
 def _dense(t):

@@ -299,3 +299,22 @@ def test_a_cleared_state_is_freed():
     with pytest.raises(L.RfxError):
         opt.step()
     assert torch.equal(p.detach(), before)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_stride_of_a_size_1_dimension_means_nothing(bits):
+    """a state from a run whose parameter had another one there is taken as it is, and so are gradients"""
+    from remixfusion_amd.optim import AdamW
+    base = torch.linspace(-1, 1, 35, device="cuda")
+    p, q = (torch.nn.Parameter(torch.as_strided(base.clone(), (5, 1, 7), st)) for st in ((1, 99, 5), (1, 5, 5)))
+    a, b = AdamW([p], lr=0.1, state_bits=bits, seed=1), AdamW([q], lr=0.1, state_bits=bits, seed=1)
+    for it in range(4):
+        grad = torch.as_strided(torch.linspace(0, 3, 35, device="cuda"), (5, 1, 7), (1, 35, 5))
+        p.grad, q.grad = (torch.as_strided(grad.clone(), (5, 1, 7), (1, st, 5)) for st in (99, 3))
+        a.step(); b.step()
+        if it == 1:                                              # each goes on with the other's
+            one, other = (copy.deepcopy(o.state_dict()) for o in (a, b))
+            moments = other["state"][0]["exp_avg"]
+            a.load_state_dict(other); b.load_state_dict(one)
+            assert a.state[p]["exp_avg"].data_ptr() == moments.data_ptr()
+    assert torch.equal(p, q) and torch.equal(a.moments()[0][0], b.moments()[0][0])
