@@ -133,11 +133,17 @@ __device__ __forceinline__ float stepped(float p, float update, float lr_wd) {
     return p - (fabsf(p) == __builtin_inff() ? update : madd(lr_wd, p, update));
 }
 
+// A clipping factor as fp32 products take it: norms beyond 2^100 limits would make one that is subnormal there, or nothing
+struct Factor32 {
+    float f, unit;
+    __device__ explicit Factor32(double x) : f((float)(x < 0x1p-100 ? x * 0x1p100 : x)), unit(x < 0x1p-100 ? 0x1p-100f : 1.f) {}
+};
+
 // ---- 32-bit moments: fp32 throughout ------------------------------------------------------------------------------------------
 // Bound by HBM: 28 bytes an fp32 element, 41.5 million in 189 us = 6.1 TB/s (a large copy: 5.4).
-__device__ __forceinline__ void adamw_one(float& p, float g, float& m, float& v, const AwGroup& a, const AwStep& s, float c) {
+__device__ __forceinline__ void adamw_one(float& p, float g, float& m, float& v, const AwGroup& a, const AwStep& s, Factor32 c) {
     const float c1 = (float)a.c1, c2 = (float)a.c2, b1 = (float)a.b1, b2 = (float)a.b2;
-    g *= c;
+    g = g * c.f * c.unit;
     m = madd(c1, g, b1 * m);
     v = madd(c2 * g, g, b2 * v);
     p = stepped(p, s.step_size * (m / madd(sqrtf(v), s.inv_bc2, a.eps)), s.lr_wd);
@@ -192,7 +198,8 @@ __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(const AwArgs k) {
     const AwTensor& t = k.t[ti];
     const AwGroup& a = k.group[t.group];
     const AwStep s = k.dev ? k.dev[ti] : a.s;
-    const float c = a.sign * (float)clip_factor(k.clip);
+    Factor32 c(clip_factor(k.clip));
+    c.f *= a.sign;
     const int64_t base = (int64_t)((int)blockIdx.x - k.first[ti]) * AW_PIECE;
     const int len = (int)(t.n - base < AW_PIECE ? t.n - base : AW_PIECE);
     T* p = (T*)t.p + base;
@@ -536,19 +543,19 @@ __global__ __launch_bounds__(JOIN) void grad_norm_join_kernel(const double* part
 
 // the norm's pieces on the blocks that the norm had them on: what an XCD's L2 still holds of a small set is found there (1.6 million
 // gradients 5.8 us, in pieces of another size 7.4)
-template <typename T> __device__ __forceinline__ void scale_piece(T* g, int len, float c) {
+template <typename T> __device__ __forceinline__ void scale_piece(T* g, int len, Factor32 c) {
     int done = 0;
     if (((uintptr_t)g & (4 * sizeof(T) - 1)) == 0) {
         done = len & ~3;
-        for (int i = threadIdx.x * 4; i < done; i += GN_THREADS * 4) store4(g + i, load4(g + i) * c);
+        for (int i = threadIdx.x * 4; i < done; i += GN_THREADS * 4) store4(g + i, load4(g + i) * c.f * c.unit);
     }
-    for (int i = done + threadIdx.x; i < len; i += GN_THREADS) g[i] = (T)((float)g[i] * c);
+    for (int i = done + threadIdx.x; i < len; i += GN_THREADS) g[i] = (T)((float)g[i] * c.f * c.unit);
 }
 
 __global__ __launch_bounds__(GN_THREADS) void grad_scale_kernel(const GnArgs k) {
     const double f = clip_factor(k.clip);
     if (f == 1.0) return;
-    const float c = (float)f;
+    const Factor32 c(f);
     for (int piece = blockIdx.x; piece < k.pieces; piece += gridDim.x) {
         const int ti = find(k.first, k.count, piece);
         const int64_t base = (int64_t)(piece - k.first[ti]) * k.piece, n = k.t[ti].n;

@@ -318,3 +318,33 @@ def test_the_stride_of_a_size_1_dimension_means_nothing(bits):
             a.load_state_dict(other); b.load_state_dict(one)
             assert a.state[p]["exp_avg"].data_ptr() == moments.data_ptr()
     assert torch.equal(p, q) and torch.equal(a.moments()[0][0], b.moments()[0][0])
+
+
+@pytest.mark.parametrize("value,limit", [(1e37, 1.0), (3e38, 1.0), (3e38, 1e-3), (3e38, 1e-8), (1e-30, 1e-32), (1e-3, 1e-44), (1e-20, 1e-30)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norms_and_factors_at_the_ends_of_fp32(dtype, value, limit):
+    """both are formed in 64 bits: squares that no fp32 holds, a norm that none holds, a factor that is subnormal there or nothing.
+    The scaled gradient has one rounding of the factor, two of the product and one to its type, to its subnormals where it is there."""
+    from remixfusion_amd.optim import AdamW, clip_grad_norm_
+    T, n = DTYPES[dtype], 3001
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda", dtype=T))
+    g = (torch.linspace(-1, 1, n, device="cuda") * value).to(T)
+    exact = g.double()
+    norm = float((exact * exact).sum().sqrt())
+    c = min(1.0, limit / (norm + 1e-6))
+    p.grad = g.clone()
+    out = float(clip_grad_norm_(p, limit))
+    assert math.isinf(out) and out > 0 if norm > 3.4028236e38 else abs(out - norm) <= (U + 1e-12) * norm + 2.0 ** -149
+    tiny = 2.0 ** -149 if dtype == "f32" else 2.0 ** -133
+    near(p.grad, (exact * c).cpu().numpy(), (half_eps(T) + 4 * U) * (exact * c).abs().cpu().numpy() + tiny, "scaled")
+    # the step sees the same: under an eps a thousand times as large it is close to -c g / eps
+    for bits in (32, 8):
+        q = torch.nn.Parameter(torch.zeros(n, device="cuda", dtype=torch.float32))
+        q.grad = exact.float()
+        opt = AdamW([q], lr=1.0, betas=(0.0, 0.5), eps=1e3 * c * value, weight_decay=0.0, state_bits=bits, max_grad_norm=limit)
+        if c * value * 1e3 < 1e-30:
+            continue                                       # (second moments under what 32 bits hold)
+        opt.step()
+        m = exact * c
+        want = -m / (m.abs() + 1e3 * c * value)
+        near(q, want.cpu().numpy(), 32 * U * want.abs().cpu().numpy() + 2.0 ** -149, (bits, "step"))
