@@ -348,3 +348,77 @@ def test_norms_and_factors_at_the_ends_of_fp32(dtype, value, limit):
         m = exact * c
         want = -m / (m.abs() + 1e3 * c * value)
         near(q, want.cpu().numpy(), 32 * U * want.abs().cpu().numpy() + 2.0 ** -149, (bits, "step"))
+
+
+def _bytes(sizes, dtype, master, bits):
+    e = 4 if dtype == "f32" else 2
+    return sum(sizes) * (2 * e + (4 if master else 0) + (2 if bits == 8 else 8))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype,master", [("f32", False), ("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
+def test_every_kind_past_the_caches(dtype, master, bits):
+    """parameters, gradients and moments of more than 64 MB in each type and state: whole vectors, and a tensor that none fits"""
+    from remixfusion_amd.optim import AdamW
+    T = DTYPES[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(47)
+    sizes = [12_000_003, 300_001]
+    assert _bytes(sizes, dtype, master, bits) > 64 << 20
+    bufs = [torch.randn(n + 1, device="cuda", generator=gen).mul(0.3).to(T) for n in sizes]
+    ps = [torch.nn.Parameter(bufs[0][:-1]), torch.nn.Parameter(bufs[1][1:])]
+    opt = AdamW(ps, **SETTINGS[1], state_bits=bits, master_weights=master, seed=5)
+    refs = [Ref(p.detach().float().cpu().numpy(), bits, i, 5) for i, p in enumerate(ps)]
+    for it in range(2):
+        for p in ps:
+            p.grad = magnitudes(p.numel(), gen).to(T)
+        opt.step()
+        for p, ref in zip(ps, refs):
+            tp, tm, tv = ref.step(p.grad.float().cpu().numpy(), **SETTINGS[1], half=U if master else half_eps(T))
+            st = opt.state[p]
+            if bits == 8:
+                _finite_runs(st, ref, it)
+            else:
+                near(st["exp_avg"], ref.m, tm, "m"); near(st["exp_avg_sq"], ref.v, tv, "v")
+                ref.m, ref.v = (st[k].double().cpu().numpy() for k in ("exp_avg", "exp_avg_sq"))
+            near(st["master"] if master else p, ref.p, tp, "p")
+            if master:
+                assert torch.equal(p.detach(), st["master"].to(T))
+            ref.p = (st["master"] if master else p.detach()).double().cpu().numpy()
+
+
+@pytest.mark.parametrize("kind", ["adamw", "adamw8bit"])
+def test_every_element_of_a_map_iteration_is_the_formula(kind):
+    """one iteration's step of the mapper's parameters against AdamW in fp64 from the same moments, however small their second moments:
+    an entry of the table that nothing has met stays what it is"""
+    from test_mapper_adamw_gpu import _pipeline, _run
+    pipe = _pipeline(optimizer=kind, grad_clip=0.5)
+    _run(pipe, 7)
+    opt, d = pipe.slam.map_optimizer, pipe.mapper._direct_iterations()
+    batch = pipe.dataset[6]
+    rays = torch.cat([batch["direction"], batch["rgb"], batch["depth"][..., None]], -1).reshape(-1, 7).to(pipe.device)
+    d.map_gradients(rays, pipe.slam.est_c2w_data[0:7:pipe.config["mapping"]["keyframe_every"]].clone())
+    params = [p for g in opt.param_groups for p in g["params"]]
+    settings = [g for g in opt.param_groups for _ in g["params"]]
+    grads = [p.grad.double() for p in params]
+    old = [(p.detach().double(), m.double(), v.double()) for p, m, v in zip(params, *opt.moments())]
+    norm = float(torch.sqrt(sum((g * g).sum() for g in grads)))
+    opt.step()
+    c = min(1.0, 0.5 / (norm + 1e-6))
+    least, untouched = 2.0 ** -149, 0
+    for p, g, s, (x, m, v) in zip(params, grads, settings, old):
+        k = float(opt.state[p]["step"])
+        terms = 0.9 * m.abs() + 0.1 * g.abs() * c
+        m, v = 0.9 * m + 0.1 * g * c, 0.99 * v + 0.01 * (g * c) ** 2
+        size, root = s["lr"] / (1 - 0.9 ** k), math.sqrt(1 - 0.99 ** k)
+        den = v.sqrt() / root + s["eps"]
+        up = size * m / den
+        want = x - s["lr"] * s["weight_decay"] * x - up
+        # the parameter's own rounding, 16 u of the update, m's terms of opposite sign (4 u of each), and what fp32's subnormals leave of m and
+        # v: 4 units of 2^-149 each, a root of them next to the denominator
+        tol = U * (2 * x.abs() + want.abs() + 16 * up.abs() + 4 * size * terms / den) + 4 * least * size / den + up.abs() * 2 * math.sqrt(least) / root / den
+        near(p, want.cpu().numpy().reshape(-1), (tol + least).cpu().numpy(), (kind, tuple(p.shape)))
+        if s["weight_decay"] == 0.0:
+            still = terms == 0
+            untouched += int(still.sum())
+            assert torch.equal(p.detach()[still], x[still].float())
+    assert untouched > 1000
