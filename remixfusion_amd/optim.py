@@ -248,7 +248,8 @@ class AdamW(torch.optim.AdamW):
                     memory and 16 instead of 28 bytes of traffic per fp32 parameter; state[p] holds uint8 "exp_avg", "exp_avg_sq" and
                     int8 "exponents" [2, ceil(n / 256)].  Rounded stochastically from a hash of (seed, step, parameter, element): the same
                     run gives the same bits.  A value that is not finite makes its 256 neighbours NaN at the next step.
-    master_weights  bfloat16 / float16 parameters are stepped in an fp32 copy, state[p]["master"], and rounded once.
+    master_weights  bfloat16 / float16 parameters are stepped in an fp32 copy, state[p]["master"], and rounded once.  What writes the
+                    parameter otherwise has to write that copy, too (or remove it: the next step makes it from the parameter).
     seed            of the 8-bit roundings.
     max_grad_norm   scale the gradients by min(1, max_grad_norm / (N + 1e-6)), N their global 2-norm, on the way into the moments: the
                     gradients themselves stay as they are.  `grad_norm` is N of the last step (fp32 scalar on the device; None where
@@ -412,6 +413,8 @@ class AdamW(torch.optim.AdamW):
                 if w is not None and tuple(w.shape) != tuple(p.shape):
                     raise _lib.RfxError(f"master of shape {tuple(w.shape)} for a parameter of shape {tuple(p.shape)}")
                 st["master"] = torch.empty_like(st["exp_avg"], dtype=torch.float32).copy_(p if w is None else w)
+        else:
+            st.pop("master", None)                           # steps without it leave it behind the parameter
 
     def _new_state(self, p, g):
         st = self.state[p]

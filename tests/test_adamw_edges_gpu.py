@@ -422,3 +422,28 @@ def test_every_element_of_a_map_iteration_is_the_formula(kind):
             untouched += int(still.sum())
             assert torch.equal(p.detach()[still], x[still].float())
     assert untouched > 1000
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_master_weights_that_come_and_go(bits):
+    """steps without the fp32 copy move the parameter past it: switched on again, it starts from the parameter; so does a removed one"""
+    from remixfusion_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(700, device="cuda", dtype=torch.bfloat16))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], lr=0.25, betas=(0.5, 0.5), weight_decay=0.0, state_bits=bits, master_weights=True)
+    held = lambda: "master" in opt.state[p]                                              # noqa: E731
+    opt.step()
+    assert held() and float(p.detach()[0]) == 0.75
+    opt.param_groups[0]["master_weights"] = False
+    for want in (0.5, 0.25):
+        opt.step()
+        assert not held() and abs(float(p.detach()[0]) - want) < 0.04           # (a moment of one byte is off by a sixteenth at most)
+    opt.param_groups[0]["master_weights"] = True
+    before = p.detach().float().clone()
+    opt.step()
+    assert held() and float((before - p.detach().float() - 0.25).abs().max()) < 0.04
+    with torch.no_grad():
+        p.fill_(4.0)
+    del opt.state[p]["master"]
+    opt.step()
+    assert held() and float((p.detach().float() - 3.75).abs().max()) < 0.04
