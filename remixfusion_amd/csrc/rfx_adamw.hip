@@ -11,8 +11,8 @@
 namespace rfx {
 
 constexpr int AW_THREADS = 256;
-// Elements per block: four a thread, one run of the 8-bit form a wave.  Small blocks fill the chip early and leave no tail: against 4096
-// elements, 135 000 parameters in 8 bits step in 5 us instead of 9, and 41.5 million in 32 bits in 191 us instead of 206.
+// Elements per block: four a thread, one run of the 8-bit form a wave.  Small blocks fill the chip early and leave no tail: 135 000 parameters
+// in 8 bits step in 4.6 us, with 4096 elements a block in 6.3; 41.5 million in 32 bits in 189 us, with 4096 in 205.
 constexpr int AW_PIECE = AW_THREADS * 4;
 constexpr int AW_TENSORS = 48;          // descriptors per launch: the kernel's arguments stay under 4 KB
 constexpr int AW_GROUPS = 8;
@@ -101,7 +101,8 @@ template <bool STREAM = false, typename T> __device__ __forceinline__ void store
     if (STREAM) __builtin_nontemporal_store(y, at); else *at = y;
 }
 
-// xor-shift / multiply mixer of 32-bit integers (a bijection)
+// xor-shift / multiply mixer of 32-bit integers (a bijection): shifts and multipliers as published by C. Wellons in 2018, the least biased of
+// the two-multiply mixers that he searched
 __host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
     x ^= x >> 16; x *= 0x7feb352dU;
     x ^= x >> 15; x *= 0x846ca68bU;
@@ -238,15 +239,16 @@ __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(const AwArgs k) {
 
 // ---- 8-bit moments ------------------------------------------------------------------------------------------------------------
 // A wave owns a run of 256 elements, four consecutive ones a lane.  The moments are formed in fp64 (full rate on this chip), so
-// that which side of a border they fall on does not depend on the order of the operations; the update is fp32.
+// that which side of a border they fall on does not depend on the order of the operations; the update is fp32 (of wide runs fp64).
 //   decode: a byte's seven (eight) bits moved to an fp32's exponent and mantissa ARE the format, subnormals included, times a power
 //           of two that is a constant of the run (beta goes into it: a product with a power of two is exact);
 //   encode: the moment times the inverse power of two, rounded to fp32 (subnormals included), leaves 20 bits below the format's
 //           last place: 16 random bits (and half of their unit) are added, and the upper bits are the code.
 // Why at random: one step moves an average by (1 - beta) of its distance -- a thousandth for beta2 = 0.999 -- and the formats' places
 // are an eighth apart; to nearest, the average would stand still.  Why second moments never become 0: m / eps would be a leap.
-// 16 bytes an fp32 element and 72 vector instructions: 41.5 million in 105-111 us = 6.0-6.3 TB/s; below some millions, where all of it
-// stays in the caches, the instructions bound it (3 million fp16 parameters, 30 MB: 12 us).  The codes are read and written through the
+// 16 bytes an fp32 element and 76 vector instructions: 41.5 million in 105-111 us = 6.0-6.3 TB/s, of them 80 us of instructions (4.9e7 a
+// launch over 1024 SIMDs at four cycles each).  3 million fp16 parameters, 30 MB that the caches hold: 12 us, of them 6 of instructions and
+// the rest the launch's own rise and fall (a CU is busy for 8.6).  The codes are read and written through the
 // caches also where the rest goes past them: four bytes a lane, they share their lines with other waves.
 __device__ __forceinline__ double pow2(int e) { return __longlong_as_double((long long)(e + 1023) << 52); }
 
@@ -573,6 +575,8 @@ static int elem_bytes(int dtype) { return dtype == RFX_F32 ? 4 : 2; }
 // Measured, us a step (plain loads and stores / past the caches), sets of fp32 tensors stepped again and again: 26 MB 9.6 / 11.0, 64 MB
 // 19 / 22, 128 MB 43 / 39, 664 MB 217 / 191; behind other work on 256 MB, as in a training loop: 16 MB 13.6 / 7.6, 64 MB 37 / 22, 128 MB
 // 64 / 40.  What is stepped next to nothing else stays in the caches under this size, and the larger sets gain either way.
+// In the mapper, whose smallest table is 26 MB by this count, behind a render and its backward: 8.6 us plain and 9.9 past the caches in 32
+// bits, 8.9 and 8.5 in 8; whole runs 2 109 and 2 082 frames/s in 32 bits, 2 086 and 2 083 in 8: under the size, plain.
 constexpr int64_t STREAM_BYTES = 64 << 20;
 static int64_t pieces_of(int64_t n) { return (n + AW_PIECE - 1) / AW_PIECE; }
 constexpr int64_t AW_BLOCKS = 0xffffffffLL / AW_THREADS;                   // of a launch: its threads are counted in 32 bits
