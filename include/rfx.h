@@ -734,9 +734,9 @@ int rfx_adam_step(const rfx_adam_tensor* tensors, int count, rfx_stream stream);
  *   exp_avg_sq        5 bits f, 3 bits n:   n 2^(E-33) if f = 0, else (8+n) 2^(E-34+f)
  * E = floor(log2(largest magnitude of the run)), one more where the significand is >= 1.875; the byte holds E of exp_avg, and of
  * exp_avg_sq -- whose range is twice as wide -- E / 2, rounded up; clamped to [-127, 127].  The byte -128: the run held a value
- * that is not finite, and all of it reads as NaN (in the call that meets it the others still step).  A moment is rounded to 20 bits below the last place
- * and then up with the probability of the rest, from 16 bits of a hash of (seed, step, index, run, element); a second moment
- * > 0 never becomes 0.  The step itself uses the moments before they are rounded.                                          */
+ * that is not finite, and all of it reads as NaN (in the call that meets it the others still step).  A moment is rounded
+ * to 20 bits below the last place and then up with the probability of the rest, from 16 bits of a hash of (seed, step,
+ * index, run, element); a second moment > 0 never becomes 0.  The step itself uses the moments before they are rounded.     */
 #define RFX_F32  0
 #define RFX_BF16 1
 #define RFX_F16  2
