@@ -485,7 +485,8 @@ class AdamW(torch.optim.AdamW):
         """plans for (parameter, its place in the optimizer, its group): states made or checked, one plan per device"""
         capturing = torch.cuda.is_current_stream_capturing()
         stepped = {p for p, _, _ in every}
-        by_device, held = {}, {t.data_ptr() for p, st in self.state.items() if p not in stepped and isinstance(st, dict) for _, t in self._tensors(st)}
+        by_device = {}
+        held = {t.data_ptr() for p, st in self.state.items() if p not in stepped and isinstance(st, dict) for _, t in self._tensors(st)}
         for g in self.param_groups:                           # (whose settings may have been changed in place)
             self._check_group(g)
         for entry in every:
